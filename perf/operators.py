@@ -5,8 +5,9 @@ A plane-record tensor is ``[N][planes][H][W][record]``: 16 bf16 or 8 fp32 channe
 ``c // record``; record slots past the channel count hold zeros.  Per-channel vectors are padded to a multiple of 32.
 
 The 8-bit states are e4m3 codes with one fp32 scale per 256 consecutive elements of a tensor (value = code * scale).  The
-scale is the block's largest magnitude over 448; a magnitude is rounded up or down at random in proportion (16 bits of a
-hash of element, step and seed), a second moment above zero keeps at least the smallest code.
+scale is the smallest power of two that brings the block's largest magnitude to 448 or below; a magnitude is rounded up or
+down at random in proportion (16 bits of a hash of element, step and seed), a second moment above zero keeps at least the
+smallest code.
 """
 import math
 import random
@@ -167,7 +168,7 @@ def prepare(case, seed):
             s["m"], s["v"] = m, v
         else:
             for name, x in (("m", m.view(-1, BLOCK)), ("v", v.view(-1, BLOCK))):
-                scale = x.abs().amax(1) / TOP
+                scale = torch.exp2(torch.ceil(torch.log2(x.abs().amax(1) / TOP)))
                 s[name] = (x / scale[:, None]).clamp(-TOP, TOP).to(torch.float8_e4m3fn).view(-1)
                 s[name + "_scale"] = scale
             positive = (v > 0) & (s["v"].float() == 0)
@@ -358,9 +359,11 @@ def _plain_adamw(s):
         bits = _hash((index + number * 0xC2B2AE35) & 0xFFFFFFFF, t, s["seed"]).view(-1, BLOCK)
         del index, number
         for name, x, b in (("m", m, bits & 0xFFFF), ("v", v, bits >> 16)):
-            scale = (x.abs().amax(1) / TOP).float()
-            inverse = torch.where(scale > 0, 1.0 / scale.double(), torch.zeros_like(scale, dtype=torch.float64))
-            y = (x.abs() * inverse[:, None]).float()
+            y = x.abs().float()
+            fraction, exponent = torch.frexp(y.amax(1))            # fraction in [0.5, 1); 448 = 0.875 * 2 ** 9
+            exponent = (exponent - torch.where(fraction <= 0.875, 9, 8)).clamp(min=-126)
+            scale = torch.where(fraction > 0, torch.ldexp(torch.ones_like(fraction), exponent), torch.zeros_like(fraction))
+            y = y * torch.ldexp(torch.ones_like(fraction), -exponent)[:, None]
             code = _encode(y, b, (x > 0) & (scale > 0)[:, None] if name == "v" else torch.zeros_like(x, dtype=torch.bool))
             code = torch.where(x < 0, code + 128, code)
             s[name], s[name + "_scale"] = code.to(torch.uint8).view(torch.float8_e4m3fn).view(-1), scale
@@ -449,8 +452,9 @@ def _exact_adamw(s):
             key = key ^ (key >> 16)
             for name, chance in (("m", key % 65536), ("v", key // 65536)):
                 x = torch.nn.functional.pad(moments[name], (0, -n % BLOCK)).view(-1, BLOCK)
-                scale = (x.abs().max(1).values / TOP).float()
-                ratio = (x.abs() / scale.double().clamp(min=1e-300)[:, None]).flatten()[:n].float().double()
+                biggest = x.abs().max(1).values
+                scale = 2.0 ** torch.ceil(torch.log2(biggest / TOP)) * (biggest > 0)
+                ratio = (x.abs() / scale.clamp(min=1e-300)[:, None]).flatten()[:n].float().double()
                 exponent = torch.floor(torch.log2(ratio.clamp(min=2.0 ** -6)))
                 exponent = exponent - (2.0 ** exponent > ratio.clamp(min=2.0 ** -6)).double()
                 unit = 2.0 ** (exponent - 3)
@@ -459,7 +463,7 @@ def _exact_adamw(s):
                 if name == "v":
                     value = torch.where(moments[name] > 0, value.clamp(min=2.0 ** -9), value)
                 out[name][own_rows] = torch.where(moments[name] < 0, -value, value)
-                out[name + "_scale"][at // BLOCK:at // BLOCK + scale.numel()] = scale.double()
+                out[name + "_scale"][at // BLOCK:at // BLOCK + scale.numel()] = scale
         else:
             out["m"][own_rows], out["v"][own_rows] = moments["m"], moments["v"]
         step = moments["m"] / (1.0 - BETA1 ** t) / ((moments["v"] / (1.0 - BETA2 ** t)).sqrt() + ADAM_EPS)
