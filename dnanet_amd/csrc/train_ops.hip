@@ -727,7 +727,13 @@ __global__ __launch_bounds__(256) void adam_kernel(float* __restrict__ p, float*
     const float vv = fmaf(beta2, v[i], (1.f - beta2) * gv * gv);
     m[i] = mv;
     v[i] = vv;
-    p[i] = pv - lr_over_bc1 * mv / (sqrtf(vv) * inv_sqrt_bc2 + eps);
+    float denom;
+    {
+#pragma clang fp contract(off)      // product and sum rounded separately, whatever instructions the build may use
+      denom = sqrtf(vv) * inv_sqrt_bc2;
+      denom = denom + eps;
+    }
+    p[i] = pv - lr_over_bc1 * mv / denom;
     if (zero_grad) g[i] = 0.f;
   }
 }
