@@ -1,0 +1,426 @@
+// AdamW over many tensors at once, moments in fp32 or in 8 bits, and the global gradient norm.
+//
+//   g' = coef * g                      coef = min(1, max_norm / (norm + 1e-6)) of the global norm, or 1
+//   m = beta1 m + (1 - beta1) g'       v = beta2 v + (1 - beta2) g'^2
+//   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+//
+// A launch takes up to ADAMW_MAX tensors BY VALUE in its kernel arguments: no table in device memory has to be kept, copied
+// or protected from a later call, and a captured launch carries its own.  The moments of all tensors lie in two flat buffers;
+// a tensor's start there is a multiple of 256 elements.
+//
+// 8-bit moments: e4m3 codes and one fp32 scale per 256 consecutive elements of a tensor, the smallest power of two that brings
+// the block's largest magnitude to 448 or below (a power of two: dividing by it rounds nothing, so a code depends on the new
+// moment alone).  Rounding is stochastic, up with the probability of the remainder, 16 bits of a hash of
+// (place in the moment buffers, step, seed) for each moment: to nearest, a second moment would stand still as soon as one step moves it by less than half a code step
+// (2^-4 of its value, where 1 - beta2 is 2^-10).  A second moment above zero keeps at least the smallest code: m / (0 + eps)
+// would be a step of any size.  New moments are formed in fp64 before they are rounded to 8 bits, so that which side of a
+// code border a value falls on does not depend on how the products were contracted.  A moment that is not finite keeps its
+// element to itself: it is left out of the block's scale and stored as NaN.
+#include <algorithm>
+#include <cmath>
+#include "common.h"
+#include "dnanet_hip.h"
+
+namespace {
+
+constexpr int ADAMW_MAX = 96;                 // tensors of a launch: their records fill the 4-KiB kernel argument segment
+constexpr int ADAMW_THREADS = 256;
+constexpr int ADAMW_CHUNK = 4096;             // elements of a block: a multiple of the 256-element state blocks
+constexpr unsigned ADAMW_P_BF16 = 1, ADAMW_G_BF16 = 2, ADAMW_VECTOR = 4;
+
+struct AdamwEntry {                           // 40 bytes
+  void* p;
+  void* g;
+  long n;
+  unsigned state;                             // start in the moment buffers / 256
+  float decay;
+  unsigned block0;                            // first block of this tensor
+  unsigned flags;
+};
+struct AdamwList {
+  AdamwEntry e[ADAMW_MAX];
+  int count;
+};
+struct AdamwArgs {
+  float beta1, beta2, omb1, omb2, eps;        // omb = 1 - beta, formed in fp64
+  double dbeta1, dbeta2, domb1, domb2;
+  float lr, step_size, inv_sqrt_bc2;          // lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t)
+  unsigned step, seed;
+  int zero_grad;
+  const float* coef;                          // nullable: [1] of {norm, coefficient}
+  const float* hyper;                         // nullable: {lr, lr / bc1, 1 / sqrt(bc2)} in device memory
+  const long long* step_dev;                  // with hyper
+};
+
+// index of the tensor that owns block b: blocks of a tensor are consecutive, block0 ascends
+__device__ __forceinline__ int adamw_find(const AdamwList& l, unsigned b) {
+  int lo = 0, hi = l.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (l.e[mid].block0 <= b) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ unsigned adamw_hash(unsigned x) {
+  x = (x ^ (x >> 16)) * 0x7FEB352Du;
+  x = (x ^ (x >> 15)) * 0x846CA68Bu;
+  return x ^ (x >> 16);
+}
+
+// four elements from index i; where the tensor is not aligned or ends, one by one
+template <typename T> __device__ __forceinline__ void adamw_load(const void* base, long i, int count, bool vec, float* f) {
+  const T* q = (const T*)base + i;
+  if (vec && count == 4) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 v = *(const float4*)q;
+      f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+    } else {
+      const uint2 v = *(const uint2*)q;
+      f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
+      f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = j < count ? dn_to_float(q[j]) : 0.f;
+  }
+}
+template <typename T> __device__ __forceinline__ void adamw_store(void* base, long i, int count, bool vec, const float* f) {
+  T* q = (T*)base + i;
+  if (vec && count == 4) {
+    if constexpr (sizeof(T) == 4) {
+      *(float4*)q = make_float4(f[0], f[1], f[2], f[3]);
+    } else {
+      const __bf16 h[4] = {(__bf16)f[0], (__bf16)f[1], (__bf16)f[2], (__bf16)f[3]};      // to nearest even
+      uint2 v;
+      v.x = (unsigned)__builtin_bit_cast(unsigned short, h[0]) | ((unsigned)__builtin_bit_cast(unsigned short, h[1]) << 16);
+      v.y = (unsigned)__builtin_bit_cast(unsigned short, h[2]) | ((unsigned)__builtin_bit_cast(unsigned short, h[3]) << 16);
+      *(uint2*)q = v;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < count) q[j] = dn_from_float<T>(f[j]);
+  }
+}
+__device__ __forceinline__ void adamw_load_any(const void* base, bool bf16, long i, int count, bool vec, float* f) {
+  if (bf16) adamw_load<__bf16>(base, i, count, vec, f); else adamw_load<float>(base, i, count, vec, f);
+}
+__device__ __forceinline__ void adamw_store_any(void* base, bool bf16, long i, int count, bool vec, const float* f) {
+  if (bf16) adamw_store<__bf16>(base, i, count, vec, f); else adamw_store<float>(base, i, count, vec, f);
+}
+
+struct AdamwScalars { float lr, step_size, inv_sqrt_bc2, coef; unsigned step; };
+__device__ __forceinline__ AdamwScalars adamw_scalars(const AdamwArgs& a) {
+  AdamwScalars s{a.lr, a.step_size, a.inv_sqrt_bc2, 1.f, a.step};
+  if (a.hyper) { s.lr = a.hyper[0]; s.step_size = a.hyper[1]; s.inv_sqrt_bc2 = a.hyper[2]; s.step = (unsigned)*a.step_dev; }
+  if (a.coef) s.coef = a.coef[1];
+  return s;
+}
+
+__global__ __launch_bounds__(ADAMW_THREADS) void adamw_kernel(AdamwList list, float* exp_avg, float* exp_avg_sq, AdamwArgs a) {
+  const int t = adamw_find(list, blockIdx.x);
+  const AdamwEntry e = list.e[t];
+  const AdamwScalars s = adamw_scalars(a);
+  const bool pb = e.flags & ADAMW_P_BF16, gb = e.flags & ADAMW_G_BF16, vec = e.flags & ADAMW_VECTOR;
+  const float keep = 1.f - s.lr * e.decay;
+  float* m = exp_avg + (long)e.state * 256;
+  float* v = exp_avg_sq + (long)e.state * 256;
+  const long lo = (long)(blockIdx.x - e.block0) * ADAMW_CHUNK, hi = min(e.n, lo + ADAMW_CHUNK);
+  for (long i = lo + threadIdx.x * 4; i < hi; i += ADAMW_THREADS * 4) {
+    const int count = (int)min(4L, hi - i);
+    float fp[4], fg[4], fm[4], fv[4];
+    adamw_load_any(e.p, pb, i, count, vec, fp);
+    adamw_load_any(e.g, gb, i, count, vec, fg);
+    adamw_load<float>(m, i, count, true, fm);
+    adamw_load<float>(v, i, count, true, fv);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float g = fg[j] * s.coef;
+      fm[j] = fmaf(a.beta1, fm[j], a.omb1 * g);
+      fv[j] = fmaf(a.beta2, fv[j], a.omb2 * g * g);
+      fp[j] = fp[j] * keep - s.step_size * fm[j] / (sqrtf(fv[j]) * s.inv_sqrt_bc2 + a.eps);
+    }
+    adamw_store_any(e.p, pb, i, count, vec, fp);
+    adamw_store<float>(m, i, count, true, fm);
+    adamw_store<float>(v, i, count, true, fv);
+    if (a.zero_grad) {
+      const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+      adamw_store_any(e.g, gb, i, count, vec, zero);
+    }
+  }
+}
+
+// magnitude over the block's scale -> e4m3 code, rounded up where the 16 random bits say so
+__device__ __forceinline__ unsigned adamw_encode(float y, unsigned bits) {
+  const bool small = y < 0.015625f;                    // below the smallest normal value (2^-6) the code steps are even: 2^-6 + y has
+  const float z = small ? y + 0.015625f : y;           // the same steps as a normal number
+  const int code = (int)((__float_as_uint(z) + (bits << 4)) >> 20) - (small ? 121 * 8 : 120 * 8);
+  return (unsigned)min(code, 126);
+}
+
+// the block's scale from its largest finite magnitude, as an exponent: the smallest k with amax <= 448 * 2^k, at least -126
+__device__ __forceinline__ int adamw_exponent(float amax) {
+  return max((int)((__float_as_uint(amax) + 0x1FFFFFu) >> 23) - 127 - 8, -126);
+}
+
+__global__ __launch_bounds__(ADAMW_THREADS) void adamw8_kernel(AdamwList list, unsigned char* exp_avg, unsigned char* exp_avg_sq,
+                                                               float* m_scale, float* v_scale, AdamwArgs a) {
+  const int t = adamw_find(list, blockIdx.x);
+  const AdamwEntry e = list.e[t];
+  const AdamwScalars s = adamw_scalars(a);
+  const bool pb = e.flags & ADAMW_P_BF16, gb = e.flags & ADAMW_G_BF16, vec = e.flags & ADAMW_VECTOR;
+  const float keep = 1.f - s.lr * e.decay;
+  const unsigned key = e.state * 256u + s.step * 0x9E3779B9u + a.seed * 0x85EBCA6Bu;
+  const long lo = (long)(blockIdx.x - e.block0) * ADAMW_CHUNK, hi = min(e.n, lo + ADAMW_CHUNK);
+  const int lane = threadIdx.x & 63;
+  // a wave owns a state block of 256 elements at a time, four per lane
+  for (long row = lo + (threadIdx.x >> 6) * 256; row < hi; row += ADAMW_THREADS * 4) {
+    const long i = row + lane * 4;
+    const int count = (int)max(0L, min(4L, hi - i));
+    const long at = (long)e.state * 256 + i;           // the state buffers hold whole blocks
+    const long block = (long)e.state + (row >> 8);
+    float fp[4], fg[4];
+    adamw_load_any(e.p, pb, i, count, vec, fp);
+    adamw_load_any(e.g, gb, i, count, vec, fg);
+    const unsigned cm = *(const unsigned*)(exp_avg + at), cv = *(const unsigned*)(exp_avg_sq + at);
+    const double ms = (double)m_scale[block] * a.dbeta1, vs = (double)v_scale[block] * a.dbeta2;
+    const float om[4] = {__builtin_amdgcn_cvt_f32_fp8(cm, 0), __builtin_amdgcn_cvt_f32_fp8(cm, 1), __builtin_amdgcn_cvt_f32_fp8(cm, 2),
+                         __builtin_amdgcn_cvt_f32_fp8(cm, 3)};
+    const float ov[4] = {__builtin_amdgcn_cvt_f32_fp8(cv, 0), __builtin_amdgcn_cvt_f32_fp8(cv, 1), __builtin_amdgcn_cvt_f32_fp8(cv, 2),
+                         __builtin_amdgcn_cvt_f32_fp8(cv, 3)};
+    float fm[4], fv[4], am = 0.f, av = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const double g = (double)fg[j] * (double)s.coef;
+      fm[j] = j < count ? (float)fma((double)om[j], ms, a.domb1 * g) : 0.f;
+      fv[j] = j < count ? (float)fma((double)ov[j], vs, a.domb2 * g * g) : 0.f;
+      const float mag = fabsf(fm[j]);
+      if (mag <= 3.4028235e38f) am = fmaxf(am, mag);
+      if (fv[j] <= 3.4028235e38f) av = fmaxf(av, fv[j]);
+    }
+#pragma unroll
+    for (int x = 32; x >= 1; x >>= 1) { am = fmaxf(am, __shfl_xor(am, x)); av = fmaxf(av, __shfl_xor(av, x)); }
+    const int em = adamw_exponent(am), ev = adamw_exponent(av);
+    const float im = __uint_as_float((unsigned)(127 - em) << 23), iv = __uint_as_float((unsigned)(127 - ev) << 23);      // 2^-k
+    unsigned om8 = 0, ov8 = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned h = adamw_hash((unsigned)(i + j) + key);
+      unsigned c = adamw_encode(fabsf(fm[j]) * im, h & 0xFFFFu);
+      if (!(fabsf(fm[j]) <= 3.4028235e38f)) c = 0x7F;
+      if (fm[j] < 0.f) c |= 0x80u;
+      om8 |= c << (8 * j);
+      c = adamw_encode(fv[j] * iv, h >> 16);
+      if (fv[j] > 0.f) c = max(c, 1u);
+      if (!(fv[j] <= 3.4028235e38f)) c = 0x7F;
+      ov8 |= c << (8 * j);
+      fp[j] = fp[j] * keep - s.step_size * fm[j] / (sqrtf(fv[j]) * s.inv_sqrt_bc2 + a.eps);
+    }
+    if (count > 0) {
+      adamw_store_any(e.p, pb, i, count, vec, fp);
+      if (a.zero_grad) {
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        adamw_store_any(e.g, gb, i, count, vec, zero);
+      }
+      *(unsigned*)(exp_avg + at) = om8;                // elements past the tensor's end are zero and stay zero
+      *(unsigned*)(exp_avg_sq + at) = ov8;
+    }
+    if (lane == 0) {
+      m_scale[block] = am > 0.f ? ldexpf(1.f, em) : 0.f;
+      v_scale[block] = av > 0.f ? ldexpf(1.f, ev) : 0.f;
+    }
+  }
+}
+
+// step counter and bias corrections in device memory, for a launch sequence that is captured and replayed
+__global__ void adamw_hyper_kernel(float* hyper, long long* step, double beta1, double beta2) {
+  if (threadIdx.x == 0 && blockIdx.x == 0) {
+    const long long t = *step + 1;
+    *step = t;
+    const double bc1 = 1.0 - pow(beta1, (double)t), bc2 = 1.0 - pow(beta2, (double)t);
+    hyper[1] = (float)((double)hyper[0] / bc1);
+    hyper[2] = (float)(1.0 / sqrt(bc2));
+  }
+}
+
+// ---- global gradient norm: squares in fp64 (no overflow, no order that matters beyond 2^-53), fixed order ------------------
+__device__ __forceinline__ double adamw_block_sum(double v) {
+  __shared__ double red[ADAMW_THREADS / 64];
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.0;
+#pragma unroll
+  for (int w = 0; w < ADAMW_THREADS / 64; ++w) v += red[w];
+  return v;
+}
+__global__ __launch_bounds__(ADAMW_THREADS) void grad_norm_kernel(AdamwList list, double* partial) {
+  const int t = adamw_find(list, blockIdx.x);
+  const AdamwEntry e = list.e[t];
+  const bool gb = e.flags & ADAMW_G_BF16, vec = e.flags & ADAMW_VECTOR;
+  const long lo = (long)(blockIdx.x - e.block0) * ADAMW_CHUNK, hi = min(e.n, lo + ADAMW_CHUNK);
+  double sum = 0.0;
+  for (long i = lo + threadIdx.x * 4; i < hi; i += ADAMW_THREADS * 4) {
+    float fg[4];
+    adamw_load_any(e.g, gb, i, (int)min(4L, hi - i), vec, fg);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum = fma((double)fg[j], (double)fg[j], sum);
+  }
+  sum = adamw_block_sum(sum);
+  if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+__global__ __launch_bounds__(ADAMW_THREADS) void grad_norm_finalize_kernel(const double* partial, long count, float max_norm, float* out) {
+  double sum = 0.0;
+  for (long i = threadIdx.x; i < count; i += ADAMW_THREADS) sum += partial[i];
+  sum = adamw_block_sum(sum);
+  if (threadIdx.x == 0) {
+    const double norm = sqrt(sum), coef = (double)max_norm / (norm + 1e-6);
+    out[0] = (float)norm;
+    out[1] = (float)(coef > 1.0 ? 1.0 : coef);         // NaN stays NaN, as the norm
+  }
+}
+
+long adamw_blocks(long n) { return (n + ADAMW_CHUNK - 1) / ADAMW_CHUNK; }
+
+int adamw_check(const char* name, const dn_adamw_tensor* t, int count, bool state) {
+  DN_CHECK_ARG(count >= 0 && (t || count == 0), "%s: null tensor list", name);
+  for (int i = 0; i < count; ++i) {
+    DN_CHECK_ARG(t[i].n >= 0 && t[i].n <= (1L << 40), "%s: tensor %d has %ld elements", name, i, t[i].n);
+    if (t[i].n == 0) continue;
+    DN_CHECK_ARG(t[i].grad && (t[i].param || !state), "%s: tensor %d: null pointer", name, i);
+    DN_CHECK_ARG((t[i].param_dtype == DN_F32 || t[i].param_dtype == DN_BF16) && (t[i].grad_dtype == DN_F32 || t[i].grad_dtype == DN_BF16),
+                 "%s: tensor %d: bad dtype", name, i);
+    const uintptr_t pa = t[i].param_dtype == DN_BF16 ? 1 : 3, ga = t[i].grad_dtype == DN_BF16 ? 1 : 3;
+    DN_CHECK_ARG(!((uintptr_t)t[i].grad & ga) && (!state || !((uintptr_t)t[i].param & pa)), "%s: tensor %d: misaligned pointer", name, i);
+    DN_CHECK_ARG(!state || (t[i].state >= 0 && t[i].state % 256 == 0 && t[i].state / 256 < (1L << 32)),
+                 "%s: tensor %d: state offset %ld is not a multiple of 256", name, i, t[i].state);
+  }
+  return DN_OK;
+}
+
+// The next launch's tensors from t[*first] on (empty ones are left out); returns its blocks, 0 when none is left
+long adamw_fill(const dn_adamw_tensor* t, int count, int* first, AdamwList* l) {
+  long blocks = 0;
+  l->count = 0;
+  while (*first < count && l->count < ADAMW_MAX) {
+    const dn_adamw_tensor& x = t[*first];
+    const long more = adamw_blocks(x.n);
+    if (blocks && blocks + more >= (1L << 31)) break;
+    if (x.n > 0) {
+      AdamwEntry& e = l->e[l->count];
+      e.p = x.param; e.g = x.grad; e.n = x.n; e.state = (unsigned)(x.state / 256); e.decay = x.weight_decay; e.block0 = (unsigned)blocks;
+      const uintptr_t pa = x.param_dtype == DN_BF16 ? 7 : 15, ga = x.grad_dtype == DN_BF16 ? 7 : 15;
+      e.flags = (x.param_dtype == DN_BF16 ? ADAMW_P_BF16 : 0) | (x.grad_dtype == DN_BF16 ? ADAMW_G_BF16 : 0) |
+                (((uintptr_t)x.param & pa) || ((uintptr_t)x.grad & ga) ? 0 : ADAMW_VECTOR);
+      ++l->count;
+      blocks += more;
+    }
+    ++*first;
+  }
+  return blocks;
+}
+
+// launches `kernel(list, ...)` over all tensors
+template <typename F> int adamw_each_launch(const dn_adamw_tensor* t, int count, F launch) {
+  AdamwList list;
+  long before = 0;
+  for (int first = 0; first < count;) {
+    const long blocks = adamw_fill(t, count, &first, &list);
+    if (!blocks) break;
+    launch(list, (unsigned)blocks, before);
+    DN_LAUNCH_CHECK();
+    before += blocks;
+  }
+  return DN_OK;
+}
+
+int adamw_run(const dn_adamw_tensor* tensors, int count, void* exp_avg, void* exp_avg_sq, float* m_scale, float* v_scale,
+              int state_bits, const AdamwArgs& a, hipStream_t st) {
+  return adamw_each_launch(tensors, count, [&](const AdamwList& list, unsigned blocks, long) {
+    if (state_bits == 8)
+      hipLaunchKernelGGL(adamw8_kernel, dim3(blocks), dim3(ADAMW_THREADS), 0, st, list, (unsigned char*)exp_avg, (unsigned char*)exp_avg_sq,
+                         m_scale, v_scale, a);
+    else
+      hipLaunchKernelGGL(adamw_kernel, dim3(blocks), dim3(ADAMW_THREADS), 0, st, list, (float*)exp_avg, (float*)exp_avg_sq, a);
+  });
+}
+
+int adamw_args(const char* name, const dn_adamw_tensor* tensors, int count, const void* exp_avg, const void* exp_avg_sq,
+               const float* m_scale, const float* v_scale, int state_bits, double beta1, double beta2, double eps, unsigned seed,
+               const float* clip, int zero_grad, AdamwArgs* a) {
+  const int rc = adamw_check(name, tensors, count, true);
+  if (rc) return rc;
+  DN_CHECK_ARG(state_bits == 32 || state_bits == 8, "%s: state_bits must be 32 or 8, got %d", name, state_bits);
+  DN_CHECK_ARG(exp_avg && exp_avg_sq && !((uintptr_t)exp_avg & 15) && !((uintptr_t)exp_avg_sq & 15),
+               "%s: moment buffers are null or not 16-byte aligned", name);
+  DN_CHECK_ARG(state_bits == 32 || (m_scale && v_scale), "%s: 8-bit moments need their scales", name);
+  DN_CHECK_ARG(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0, "%s: betas must be in [0, 1), eps must not be negative", name);
+  *a = AdamwArgs{};
+  a->beta1 = (float)beta1; a->beta2 = (float)beta2; a->omb1 = (float)(1.0 - beta1); a->omb2 = (float)(1.0 - beta2); a->eps = (float)eps;
+  a->dbeta1 = beta1; a->dbeta2 = beta2; a->domb1 = 1.0 - beta1; a->domb2 = 1.0 - beta2;
+  a->seed = seed; a->zero_grad = zero_grad; a->coef = clip;
+  return DN_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+long dn_grad_norm_workspace_bytes(const dn_adamw_tensor* tensors, int count) {
+  if (adamw_check("dn_grad_norm_workspace_bytes", tensors, count, false)) return -1;
+  long blocks = 1;
+  for (int i = 0; i < count; ++i) blocks += adamw_blocks(tensors[i].n);
+  return blocks * (long)sizeof(double);
+}
+
+int dn_grad_norm(const dn_adamw_tensor* tensors, int count, float max_norm, float* out, void* workspace, long workspace_bytes, void* stream) {
+  const long need = dn_grad_norm_workspace_bytes(tensors, count);
+  if (need < 0) return DN_ERR_ARG;
+  DN_CHECK_ARG(out && max_norm > 0.f, "dn_grad_norm: null output or max_norm not above zero");
+  DN_CHECK_ARG(workspace && !((uintptr_t)workspace & 7) && workspace_bytes >= need,
+               "dn_grad_norm: workspace of %ld bytes, %ld needed (8-byte aligned)", workspace_bytes, need);
+  double* partial = (double*)workspace;
+  const hipStream_t st = (hipStream_t)stream;
+  const int rc = adamw_each_launch(tensors, count, [&](const AdamwList& list, unsigned blocks, long before) {
+    hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(ADAMW_THREADS), 0, st, list, partial + before);
+  });
+  if (rc) return rc;
+  hipLaunchKernelGGL(grad_norm_finalize_kernel, dim3(1), dim3(ADAMW_THREADS), 0, st, partial, need / (long)sizeof(double) - 1, max_norm, out);
+  DN_LAUNCH_CHECK();
+  return DN_OK;
+}
+
+int dn_adamw_step(const dn_adamw_tensor* tensors, int count, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
+                  float* exp_avg_sq_scale, int state_bits, double lr, double beta1, double beta2, double eps, long step, unsigned seed,
+                  const float* clip, int zero_grad, void* stream) {
+  AdamwArgs a;
+  const int rc = adamw_args("dn_adamw_step", tensors, count, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, state_bits, beta1, beta2,
+                            eps, seed, clip, zero_grad, &a);
+  if (rc) return rc;
+  DN_CHECK_ARG(step >= 1, "dn_adamw_step: step %ld is below 1", step);
+  a.lr = (float)lr;
+  a.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
+  a.inv_sqrt_bc2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+  a.step = (unsigned)step;
+  return adamw_run(tensors, count, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, state_bits, a, (hipStream_t)stream);
+}
+
+int dn_adamw_step_graph(const dn_adamw_tensor* tensors, int count, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
+                        float* exp_avg_sq_scale, int state_bits, float* hyper, long long* step, double beta1, double beta2, double eps,
+                        unsigned seed, const float* clip, int zero_grad, void* stream) {
+  AdamwArgs a;
+  const int rc = adamw_args("dn_adamw_step_graph", tensors, count, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, state_bits, beta1,
+                            beta2, eps, seed, clip, zero_grad, &a);
+  if (rc) return rc;
+  DN_CHECK_ARG(hyper && step, "dn_adamw_step_graph: null hyper / step");
+  a.hyper = hyper;
+  a.step_dev = step;
+  hipLaunchKernelGGL(adamw_hyper_kernel, dim3(1), dim3(64), 0, (hipStream_t)stream, hyper, step, beta1, beta2);
+  DN_LAUNCH_CHECK();
+  return adamw_run(tensors, count, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, state_bits, a,
+                   (hipStream_t)stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,158 @@
+"""GroupNorm with an activation on plane-record tensors: the batch-independent alternative to the BatchNorm2d + ReLU of a
+``DoubleConv`` (reference ``unet_architecture.py:17,21``; a group norm has no counterpart there).
+
+``y = act(group_norm(x))`` per image over ``groups`` groups of channels, statistics in fp32 or more, and its backward pass;
+both run on the current stream of the tensors' device.  Tensors are ``PlaneBuffer.ref`` views (channels last inside 32-byte
+records, see ``include/dnanet_hip.h``), the per-channel vectors fp32.
+"""
+from __future__ import annotations
+
+from contextlib import nullcontext
+from typing import Dict, Optional, Tuple
+
+import torch
+
+from . import hip
+from .hip import DnTensor, PlaneBuffer
+
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}      # DN_ACT_*
+
+
+def parse_activation(activation: str) -> int:
+    try:
+        return ACTIVATIONS[str(activation).lower()]
+    except KeyError:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
+
+
+class GroupNormStats:
+    """What a forward pass leaves for its backward pass: ``mean`` / ``rstd`` (N, groups), the fused ``scale`` / ``shift``
+    (N, channels padded to 32), and how they were made."""
+
+    __slots__ = ("mean", "rstd", "scale", "shift", "groups", "activation")
+
+    def __init__(self, mean: torch.Tensor, rstd: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor, groups: int, activation: str):
+        self.mean, self.rstd, self.scale, self.shift = mean, rstd, scale, shift
+        self.groups, self.activation = groups, activation
+
+    @staticmethod
+    def floats(n: int, channels: int, groups: int) -> int:
+        return 2 * n * (groups + hip.channel_pad(channels))
+
+    @classmethod
+    def from_flat(cls, flat: torch.Tensor, n: int, channels: int, groups: int, activation: str) -> "GroupNormStats":
+        """Views into ``floats(n, channels, groups)`` consecutive fp32 values."""
+        pad = hip.channel_pad(channels)
+        a, b = n * groups, n * pad
+        mean, rstd, scale, shift = flat.split_with_sizes((a, a, b, b))
+        return cls(mean.view(n, groups), rstd.view(n, groups), scale.view(n, pad), shift.view(n, pad), groups, activation)
+
+
+_workspaces: Dict[Tuple[int, int], torch.Tensor] = {}
+
+
+def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+    """Zero-filled before its first use, as the library asks.  Calls on one stream follow each other and share a workspace.  A
+    call under HIP-graph capture gets one of its own inside the graph (zeroed there on every replay): two graphs captured on
+    the same stream may be replayed at the same time."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    ws = _workspaces.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = _workspaces[key] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+    return ws
+
+
+def _on(device: torch.device):
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _owner(ref: DnTensor, what: str) -> PlaneBuffer:
+    buf = getattr(ref, "_owner", None)
+    if not isinstance(buf, PlaneBuffer):
+        raise TypeError(f"{what} must be a PlaneBuffer.ref(channels, plane0)")
+    return buf
+
+
+def _same(buf: PlaneBuffer, like: PlaneBuffer, what: str):
+    if (buf.n, buf.h, buf.w, buf.dtype) != (like.n, like.h, like.w, like.dtype) or buf.data.device != like.data.device:
+        raise ValueError(f"{what} is {(buf.n, buf.h, buf.w)} {buf.data.dtype} on {buf.data.device}, x is {(like.n, like.h, like.w)} "
+                         f"{like.data.dtype} on {like.data.device}")
+
+
+def _vector(t: torch.Tensor, shape, device, what: str) -> int:
+    if t.dtype != torch.float32 or tuple(t.shape) != tuple(shape) or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous float32 tensor of shape {tuple(shape)} on {device}, got {tuple(t.shape)} {t.dtype} "
+                         f"on {t.device}")
+    return t.data_ptr()
+
+
+def _need(n: int, channels: int, h: int, w: int, groups: int, dtype: int) -> int:
+    nbytes = hip.lib.dn_group_norm_workspace_bytes(n, channels, h, w, groups, dtype)
+    if nbytes < 0:
+        raise ValueError(hip.lib.dn_last_error().decode())
+    return nbytes
+
+
+def group_norm_act(x: DnTensor, gamma: torch.Tensor, beta: torch.Tensor, groups: int, eps: float = 1e-5, activation: str = "relu",
+                   out: Optional[DnTensor] = None, stats: Optional[GroupNormStats] = None, workspace: Optional[torch.Tensor] = None
+                   ) -> Tuple[PlaneBuffer, GroupNormStats]:
+    """``act(group_norm(x, groups, gamma, beta, eps))``.  ``out`` (default: a new buffer) may be ``x`` itself; ``stats``: where
+    the statistics go (default: new tensors); ``workspace``: a caller's own (uint8, zeroed before its first use, one call at
+    a time).  Returns the output's buffer and the statistics for the backward call."""
+    src = _owner(x, "x")
+    act, c, dev = parse_activation(activation), x.channels, src.data.device
+    need = _need(src.n, c, src.h, src.w, groups, src.dtype)
+    g, b = _vector(gamma, (c,), dev, "gamma"), _vector(beta, (c,), dev, "beta")
+    if out is None:
+        dst = PlaneBuffer(src.n, hip.planes(c, src.dtype), src.h, src.w, src.dtype, dev)
+        out = dst.ref(c)
+    else:
+        dst = _owner(out, "out")
+        _same(dst, src, "out")
+    if stats is None:
+        flat = torch.empty(GroupNormStats.floats(src.n, c, groups), dtype=torch.float32, device=dev)
+        stats = GroupNormStats.from_flat(flat, src.n, c, groups, activation)
+    pad = hip.channel_pad(c)
+    vectors = [_vector(stats.mean, (src.n, groups), dev, "stats.mean"), _vector(stats.rstd, (src.n, groups), dev, "stats.rstd"),
+               _vector(stats.scale, (src.n, pad), dev, "stats.scale"), _vector(stats.shift, (src.n, pad), dev, "stats.shift")]
+    with _on(dev):
+        ws = _workspace(dev, need) if workspace is None else workspace
+        hip.check(hip.lib.dn_group_norm_act(x, out, src.n, src.h, src.w, groups, g, b, eps, act, *vectors, ws.data_ptr(), ws.numel(),
+                                            src.dtype, hip.stream_ptr()))
+    stats.groups, stats.activation = groups, activation
+    return dst, stats
+
+
+def group_norm_act_backward(g: DnTensor, x: DnTensor, gamma: torch.Tensor, stats: GroupNormStats, out: Optional[DnTensor] = None,
+                            dgamma: Optional[torch.Tensor] = None, dbeta: Optional[torch.Tensor] = None,
+                            workspace: Optional[torch.Tensor] = None) -> Tuple[PlaneBuffer, torch.Tensor, torch.Tensor]:
+    """``g`` = dL/d(output) -> (dL/dx, dL/dgamma, dL/dbeta).  ``x``, ``gamma``, ``stats``: as the forward call took and returned
+    them.  ``out`` (default: a new buffer) may be ``g`` itself, not ``x``."""
+    src, grad = _owner(x, "x"), _owner(g, "g")
+    _same(grad, src, "g")
+    c, dev, groups = x.channels, src.data.device, stats.groups
+    need = _need(src.n, c, src.h, src.w, groups, src.dtype)
+    ga = _vector(gamma, (c,), dev, "gamma")
+    if out is None:
+        dst = PlaneBuffer(src.n, hip.planes(c, src.dtype), src.h, src.w, src.dtype, dev)
+        out = dst.ref(c)
+    else:
+        dst = _owner(out, "out")
+        _same(dst, src, "out")
+        if dst.data.data_ptr() == src.data.data_ptr() and abs(out.plane0 - x.plane0) < hip.planes(c, src.dtype):
+            raise ValueError("out must not overlap x")
+    if dgamma is None:
+        dgamma = torch.empty(c, dtype=torch.float32, device=dev)
+    if dbeta is None:
+        dbeta = torch.empty(c, dtype=torch.float32, device=dev)
+    pad = hip.channel_pad(c)
+    vectors = [_vector(stats.mean, (src.n, groups), dev, "stats.mean"), _vector(stats.rstd, (src.n, groups), dev, "stats.rstd"),
+               _vector(stats.scale, (src.n, pad), dev, "stats.scale"), _vector(stats.shift, (src.n, pad), dev, "stats.shift")]
+    dg, db = _vector(dgamma, (c,), dev, "dgamma"), _vector(dbeta, (c,), dev, "dbeta")
+    with _on(dev):
+        ws = _workspace(dev, need) if workspace is None else workspace
+        hip.check(hip.lib.dn_group_norm_act_backward(g, x, out, src.n, src.h, src.w, groups, ga, *vectors, parse_activation(stats.activation),
+                                                     dg, db, ws.data_ptr(), ws.numel(), src.dtype, hip.stream_ptr()))
+    return dst, dgamma, dbeta

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_long, c_void_p
+from ctypes import POINTER, Structure, c_char_p, c_double, c_float, c_int, c_long, c_uint, c_void_p
 
 import torch
 
@@ -32,6 +32,12 @@ class DnPackJob(Structure):
     """``dn_pack_job`` of include/dnanet_hip.h."""
     _fields_ = [("w", c_void_p), ("scale", c_void_p), ("out", c_void_p), ("cout", c_int), ("cin", c_int), ("taps", c_int),
                 ("mode", c_int), ("rows_pad", c_int), ("nchunk", c_int), ("gsize", c_int), ("block0", c_int)]
+
+
+class DnAdamwTensor(Structure):
+    """``dn_adamw_tensor`` of include/dnanet_hip.h."""
+    _fields_ = [("param", c_void_p), ("grad", c_void_p), ("n", c_long), ("state", c_long), ("weight_decay", c_float),
+                ("param_dtype", c_int), ("grad_dtype", c_int), ("reserved", c_int)]
 
 
 class HipError(RuntimeError):
@@ -113,6 +119,17 @@ _SIGS = {
     "dn_conv_first_x3": (c_int, [_P, _P, _P, DnTensorX3] + [c_int] * 7 + [_P]),
     "dn_head_1x1_x3": (c_int, [DnTensorX3, _P, _P, _P, _P, c_int, c_int, c_int, _P]),
     "dn_conv_transpose_1x2_x3": (c_int, [DnTensorX3, _P, _P, DnTensorX3, c_int, c_int, c_int, _P]),
+    "dn_adamw_step": (c_int, [POINTER(DnAdamwTensor), c_int, _P, _P, _P, _P, c_int, c_double, c_double, c_double, c_double, c_long, c_uint, _P,
+                              c_int, _P]),
+    "dn_adamw_step_graph": (c_int, [POINTER(DnAdamwTensor), c_int, _P, _P, _P, _P, c_int, _P, _P, c_double, c_double, c_double, c_uint, _P,
+                                    c_int, _P]),
+    "dn_grad_norm_workspace_bytes": (c_long, [POINTER(DnAdamwTensor), c_int]),
+    "dn_grad_norm": (c_int, [POINTER(DnAdamwTensor), c_int, c_float, _P, _P, c_long, _P]),
+    "dn_group_norm_workspace_bytes": (c_long, [c_int] * 6),
+    "dn_group_norm_act": (c_int, [DnTensor, DnTensor, c_int, c_int, c_int, c_int, _P, _P, c_float, c_int, _P, _P, _P, _P, _P, c_long,
+                                  c_int, _P]),
+    "dn_group_norm_act_backward": (c_int, [DnTensor, DnTensor, DnTensor, c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P, c_int, _P, _P, _P,
+                                           c_long, c_int, _P]),
     "dn_call_alleles": (c_int, [_P, _P, _P, c_long, _P, _P, _P, c_int, c_int, c_int, c_int, _P, _P, _P]),
 }
 
@@ -253,6 +270,18 @@ class PlaneBuffer:
             self.data = arena.take(shape, torch_dtype(dtype), zero)
         else:
             self.data = (torch.zeros if zero else torch.empty)(shape, dtype=torch_dtype(dtype), device=device)
+
+    @classmethod
+    def wrap(cls, data: torch.Tensor) -> "PlaneBuffer":
+        """A buffer over existing memory: a contiguous (N, planes, H, W, record) tensor of 16 bf16 or 8 fp32 per record."""
+        dtype = {torch.bfloat16: BF16, torch.float32: F32}.get(data.dtype)
+        if dtype is None or data.dim() != 5 or data.shape[4] != epr(dtype) or not data.is_contiguous() or not data.is_cuda:
+            raise ValueError(f"expected a contiguous device tensor of records (N, planes, H, W, 16 bf16 | 8 float32), got {tuple(data.shape)} "
+                             f"{data.dtype} on {data.device}")
+        buf = cls.__new__(cls)
+        buf.n, buf.planes_total, buf.h, buf.w = data.shape[:4]
+        buf.dtype, buf.data = dtype, data
+        return buf
 
     def ref(self, channels: int, plane0: int = 0) -> DnTensor:
         assert plane0 + planes(channels, self.dtype) <= self.planes_total

@@ -252,6 +252,26 @@ int dn_bn_train_backward_apply_totals(dn_tensor g, dn_tensor y, const float* sca
                                       const float* gamma, const float* mean, const float* invstd, const double* local_totals,
                                       const double* global_totals, double count, float* dgamma, float* dbeta, float* coef,
                                       int dtype, void* stream);
+/* ---- GroupNorm with an activation (NO COUNTERPART IN THE REFERENCE, whose DoubleConv has BatchNorm2d + ReLU,
+ * unet_architecture.py:17,21: the batch-independent alternative in the same place) -------------------------------------
+ * torch.nn.functional.group_norm(x, groups, gamma, beta, eps) followed by the activation, per image and group over the
+ * group's channels and H x W.  gamma / beta: [C]; mean / rstd: [N][groups]; scale / shift: [N][dn_channel_pad(C)], zero past
+ * C: gamma * rstd and beta - mean * scale, kept for the backward pass.  C is a multiple of groups (groups need not fill
+ * records), H * W <= 2^25, eps > 0.  a may be x.  N = 0 returns without a launch.
+ * workspace: dn_group_norm_workspace_bytes (-1: refused sizes), 16-byte aligned; zero-filled by the caller before its first
+ * use, left for the next call as each call needs it.  It may serve any sizes it is large enough for, one call at a time:
+ * calls that overlap on the GPU need workspaces of their own. */
+#define DN_ACT_NONE 0
+#define DN_ACT_RELU 1
+#define DN_ACT_SILU 2   /* z * sigmoid(z) */
+long dn_group_norm_workspace_bytes(int N, int C, int H, int W, int groups, int dtype);
+int dn_group_norm_act(dn_tensor x, dn_tensor a, int N, int H, int W, int groups, const float* gamma, const float* beta, float eps, int act,
+                      float* mean, float* rstd, float* scale, float* shift, void* workspace, long workspace_bytes, int dtype, void* stream);
+/* Its backward: g = dL/da in, dx = dL/dx out (dx may be g; not x), dgamma / dbeta [C] overwritten.  mean / rstd / scale / shift as
+ * the forward call saved them; the activation's derivative is taken at x * scale + shift. */
+int dn_group_norm_act_backward(dn_tensor g, dn_tensor x, dn_tensor dx, int N, int H, int W, int groups, const float* gamma,
+                               const float* mean, const float* rstd, const float* scale, const float* shift, int act, float* dgamma,
+                               float* dbeta, void* workspace, long workspace_bytes, int dtype, void* stream);
 /* Backward of nn.MaxPool2d((1,2)) (unet_architecture.py:37) fused with the skip-connection add:
  * g = dskip (nullable .base) + route(dpool) to the first maximal element of every pair of x. */
 int dn_maxpool_1x2_backward(dn_tensor x, dn_tensor dpool, dn_tensor dskip, dn_tensor g, int N, int H, int Wout, int dtype,
@@ -302,6 +322,39 @@ int dn_adam_step(float* params, float* grads, float* exp_avg, float* exp_avg_sq,
  * scalars.  beta / eps / weight_decay are launch constants. */
 int dn_adam_step_graph(float* params, float* grads, float* exp_avg, float* exp_avg_sq, long n, float* hyper, long long* step,
                        float beta1, float beta2, float eps, float weight_decay, float grad_scale, int zero_grad, void* stream);
+/* ---- AdamW over many tensors (NO COUNTERPART IN THE REFERENCE, which has torch.optim.Adam with coupled L2,
+ * trainable_unet.py:155-157) --------------------------------------------------------------------------------------------
+ * torch.optim.AdamW: decoupled weight decay, one per tensor.  `tensors` is a HOST array, read during the call (its contents
+ * travel as kernel arguments, so a captured call keeps them); tensors must not overlap.  exp_avg / exp_avg_sq: the moments of
+ * all tensors in two flat buffers, 16-byte aligned; `state` of a tensor is its first element there, a multiple of 256, and
+ * the buffers hold whole blocks of 256.
+ *   state_bits 32: fp32.  state_bits 8: one e4m3 code per element and one fp32 scale per block of 256 (exp_avg_scale /
+ *   exp_avg_sq_scale [state / 256 + block], powers of two; value = code * scale), rounded stochastically from a hash of
+ *   (element's place in the buffers, step, seed); a moment that is not finite is stored as NaN.
+ * clip (nullable): {norm, coefficient} in device memory as dn_grad_norm writes them; gradients are multiplied by the
+ * coefficient.  zero_grad: gradients are zeroed in the same pass.  step counts from 1. */
+typedef struct dn_adamw_tensor {
+  void* param;           /* contiguous, param_dtype */
+  void* grad;            /* contiguous, grad_dtype */
+  long n;                /* elements; 0: left out */
+  long state;            /* first element in the moment buffers, a multiple of 256 */
+  float weight_decay;
+  int param_dtype, grad_dtype;   /* DN_DTYPE_F32 | DN_DTYPE_BF16 */
+  int reserved;
+} dn_adamw_tensor;
+int dn_adamw_step(const dn_adamw_tensor* tensors, int count, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
+                  float* exp_avg_sq_scale, int state_bits, double lr, double beta1, double beta2, double eps, long step, unsigned seed,
+                  const float* clip, int zero_grad, void* stream);
+/* The same for a captured and replayed launch sequence: *step (device) is incremented, hyper[0] (device) is the learning rate,
+ * hyper[1..2] receive the bias corrections (as dn_adam_step_graph). */
+int dn_adamw_step_graph(const dn_adamw_tensor* tensors, int count, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
+                        float* exp_avg_sq_scale, int state_bits, float* hyper, long long* step, double beta1, double beta2, double eps,
+                        unsigned seed, const float* clip, int zero_grad, void* stream);
+/* torch.nn.utils.clip_grad_norm_ without a visit to the host: out[0] = 2-norm of all gradients together (squares summed in
+ * fp64, fixed order), out[1] = min(1, max_norm / (out[0] + 1e-6)); the gradients are not written (dn_adamw_step scales them).
+ * workspace: dn_grad_norm_workspace_bytes, 8-byte aligned. */
+long dn_grad_norm_workspace_bytes(const dn_adamw_tensor* tensors, int count);
+int dn_grad_norm(const dn_adamw_tensor* tensors, int count, float max_norm, float* out, void* workspace, long workspace_bytes, void* stream);
 /* int16 RFU -> fp32 (get_input, trainable_unet.py:70-72). */
 int dn_i16_to_f32(const short* in, float* out, long n, void* stream);
 
