@@ -43,6 +43,8 @@ def all_reduce_sum(tensor: torch.Tensor, group=None):
 
 
 def broadcast(tensor: torch.Tensor, src: int = 0, group=None):
+    if not tensor.numel():          # a net without running statistics
+        return
     if _host_staged(tensor, group):
         host = tensor.detach().cpu()
         dist.broadcast(host, src=src, group=group)

@@ -26,6 +26,7 @@ from . import hip
 from .allele_caller import NearestBasePairCaller
 from .data import chunks
 from .prediction import Prediction
+from .optim import HipAdamW
 from .unet import ExponentialLR, GraphedTrainStep, HipAdam, HipUNet
 
 LOGGER = logging.getLogger("dnanet")
@@ -171,12 +172,15 @@ class _ResidentSet:
 
 class DNANet_UNet(TrainableModel):
     def __init__(self, depth: int, kernel_size: Tuple[int, int], num_filters: int = 64, device: Optional[str] = None,
-                 apply_allele_caller: Optional[bool] = True, dtype: str = "fp32"):
+                 apply_allele_caller: Optional[bool] = True, dtype: str = "fp32", norm: str = "batch", num_groups: int = 8,
+                 activation: str = "relu"):
         """Same keywords as the reference (``trainable_unet.py:38-58``); ``dtype`` ("fp32" | "bf16" | inference only: "bf16x3", "bf16x3@<levels>") selects
-        exact-fp32 MFMA (default, reference numerics) or bf16 MFMA with fp32 accumulation."""
+        exact-fp32 MFMA (default, reference numerics) or bf16 MFMA with fp32 accumulation.  ``norm="group"``: a group norm
+        of ``num_groups`` groups with ``activation`` ("relu" | "silu" | "none") in the place of BatchNorm + ReLU."""
         self._device = device or TORCH_DEFAULT_DEVICE
         # On a 'cpu' device only the parameter tree exists (checkpoint I/O, config plumbing); any forward raises.
-        self._model = HipUNet(depth, tuple(kernel_size), num_filters, self._device, dtype=dtype)
+        self._model = HipUNet(depth, tuple(kernel_size), num_filters, self._device, dtype=dtype, norm=norm,
+                              num_groups=num_groups, activation=activation)
         self.loss_fn = self._dice
         self.allele_caller = NearestBasePairCaller() if apply_allele_caller else None
         self._resident: Optional[_ResidentSet] = None
@@ -263,7 +267,9 @@ class DNANet_UNet(TrainableModel):
                 raise TypeError("`validation_set` is required when `save_best` is True")
             if checkpoint_dir is None:
                 raise TypeError("`checkpoint_dir` is required when `save_best` is True")
-        optimizer = HipAdam(self._model, lr=learning_rate, weight_decay=weight_decay)
+        # ``optimizer="adam"`` (the reference's, coupled L2) | "adamw" | "adamw8bit" (decoupled decay of the weights, fp32 or
+        # 8-bit moments); ``max_grad_norm`` (the AdamW forms): gradients clipped to a global norm
+        optimizer = self._make_optimizer(kwargs.pop("optimizer", "adam"), learning_rate, weight_decay, kwargs.pop("max_grad_norm", None))
         scheduler = None
         if use_scheduler:
             LOGGER.info(f"Setting up exponential scheduler, starting with learning rate {learning_rate}")
@@ -307,6 +313,8 @@ class DNANet_UNet(TrainableModel):
         sync_bn = bool(kwargs.pop("sync_bn", False))
         if sync_bn and not dp:
             raise ValueError("sync_bn needs data_parallel training (an initialised process group)")
+        if sync_bn and self._model.norm == "group":
+            raise ValueError("sync_bn: norm 'group' has no batch statistics to synchronise")
         self._dp = {"trainer": None, "sync_bn": sync_bn} if dp else None
         use_graph = kwargs.pop("hip_graph", None)
         if use_graph is None:
@@ -335,6 +343,16 @@ class DNANet_UNet(TrainableModel):
             else:
                 shutil.rmtree(checkpoint_dir / "best_model")
             LOGGER.info("Restored previous best model")
+
+    def _make_optimizer(self, name: str, learning_rate: float, weight_decay: float, max_grad_norm: Optional[float]):
+        if name == "adam":
+            if max_grad_norm is not None:
+                raise ValueError("max_grad_norm needs optimizer 'adamw' or 'adamw8bit'")
+            return HipAdam(self._model, lr=learning_rate, weight_decay=weight_decay)
+        if name in ("adamw", "adamw8bit"):
+            return HipAdamW(self._model, lr=learning_rate, weight_decay=weight_decay, state_bits=8 if name == "adamw8bit" else 32,
+                            max_grad_norm=max_grad_norm)
+        raise ValueError(f"optimizer must be 'adam', 'adamw' or 'adamw8bit', got {name!r}")
 
     def _fit_epochs(self, dataset, validation_set, num_epochs, steps_per_epoch, steps_per_epoch_val, batch_size, optimizer,
                     scheduler, metrics, writer, save_best, checkpoint_dir, min_delta, prev_best, best_validation_loss):

@@ -37,8 +37,9 @@ class UpUnit:
     level: int     # level of its OUTPUT
 
 
-def unet_layout(depth: int, kernel_size: Sequence[int], num_filters: int):
-    """Ordered parameter spec [(key, shape, kind)] and the unit lists, in module order."""
+def unet_layout(depth: int, kernel_size: Sequence[int], num_filters: int, norm: str = "batch"):
+    """Ordered parameter spec [(key, shape, kind)] and the unit lists, in module order.  ``norm="group"``: a group norm in the
+    place of every BatchNorm (the same keys without running statistics and batch count)."""
     kh, kw = int(kernel_size[0]), int(kernel_size[1])
     spec: List[Tuple[str, Tuple[int, ...], str]] = []
     convs: List[ConvUnit] = []
@@ -51,9 +52,10 @@ def unet_layout(depth: int, kernel_size: Sequence[int], num_filters: int):
             spec.append((c + ".bias", (cout,), "param"))
             spec.append((b + ".weight", (cout,), "param"))
             spec.append((b + ".bias", (cout,), "param"))
-            spec.append((b + ".running_mean", (cout,), "stat"))
-            spec.append((b + ".running_var", (cout,), "stat"))
-            spec.append((b + ".num_batches_tracked", (), "count"))
+            if norm == "batch":
+                spec.append((b + ".running_mean", (cout,), "stat"))
+                spec.append((b + ".running_var", (cout,), "stat"))
+                spec.append((b + ".num_batches_tracked", (), "count"))
             convs.append(ConvUnit(c, b, c_in, cout, level, sp))
 
     cin = 1
@@ -91,10 +93,10 @@ def _numel(shape):
 class ParameterTree(nn.Module):
     """Registers every state_dict entry as a view into a flat arena, on ``device``."""
 
-    def __init__(self, depth: int, kernel_size: Sequence[int], num_filters: int, device):
+    def __init__(self, depth: int, kernel_size: Sequence[int], num_filters: int, device, norm: str = "batch"):
         super().__init__()
         self.depth, self.kernel_size, self.num_filters = depth, (int(kernel_size[0]), int(kernel_size[1])), num_filters
-        spec, self.conv_units, self.up_units = unet_layout(depth, kernel_size, num_filters)
+        spec, self.conv_units, self.up_units = unet_layout(depth, kernel_size, num_filters, norm)
         self.spec = spec
         n_param = sum(_numel(s) for _, s, k in spec if k == "param")
         n_stat = sum(_numel(s) for _, s, k in spec if k == "stat")

@@ -17,11 +17,13 @@ import os
 import torch
 
 from . import hip
+from .group_norm import GroupNormStats, group_norm_act, group_norm_act_backward, parse_activation
 from .hip import BF16, F32, PlaneBuffer, StepArena
 from .params import ConvUnit, ParameterTree
 
 BN_EPS = 1e-5       # nn.BatchNorm2d default used by the reference (unet_architecture.py:17,21)
 BN_MOMENTUM = 0.1
+GN_EPS = 1e-5       # torch.nn.GroupNorm's default (norm="group")
 
 _DTYPES = {"fp32": F32, "float32": F32, "f32": F32, "bf16": BF16, "bfloat16": BF16}
 
@@ -56,14 +58,28 @@ class HipUNet(ParameterTree):
 
     MAX_CHUNK = 256     # profiles per inference pass (eval-mode BN is batch independent)
 
-    def __init__(self, depth: int, kernel_size: Sequence[int], num_filters: int, device, dtype="fp32"):
-        super().__init__(depth, kernel_size, num_filters, device)
+    def __init__(self, depth: int, kernel_size: Sequence[int], num_filters: int, device, dtype="fp32", norm: str = "batch",
+                 num_groups: int = 8, activation: str = "relu"):
+        """``norm="batch"``: the reference's BatchNorm2d + ReLU.  ``norm="group"``: a group norm of ``num_groups`` groups and
+        ``activation`` ("relu" | "silu" | "none") after every convolution -- the same arithmetic in training and evaluation,
+        independent of the batch and of how a batch is spread over ranks."""
+        if norm not in ("batch", "group"):
+            raise ValueError(f"norm must be 'batch' or 'group', got {norm!r}")
+        parse_activation(activation)
+        if norm == "batch" and activation != "relu":
+            raise ValueError("norm 'batch' is followed by relu; other activations need norm 'group'")
+        super().__init__(depth, kernel_size, num_filters, device, norm)
         if num_filters % 8:
             raise ValueError("num_filters must be a multiple of 8 for the MI355X kernels")
+        if norm == "group" and (num_groups < 1 or num_filters % num_groups):
+            raise ValueError(f"num_filters {num_filters} does not divide into {num_groups} groups")
+        self.norm, self.num_groups, self.activation = norm, int(num_groups), activation
         self.dtype = parse_dtype(dtype)
         self.split_levels = parse_split_levels(dtype, depth)       # > 0: the bf16x3 inference mode on that many levels
         if self.split_levels and tuple(kernel_size) not in ((3, 5), (1, 3)):
             raise ValueError("dtype bf16x3 is built for kernel_size (3, 5) and (1, 3)")
+        if self.split_levels and norm == "group":
+            raise ValueError("dtype bf16x3 folds BatchNorm into the weights: it has no norm 'group' form")
         self._eval_cache = None
         self._eval_cache_version = None
         self.profile = None     # set to a list to collect (kernel tag, flops, start event, end event) per conv launch
@@ -81,7 +97,7 @@ class HipUNet(ParameterTree):
         # units on the main stream.  DN_TUNE_NO_WGRAD_STREAM=1 keeps everything on one stream (A/B switch).
         self.overlap_wgrad = self.flat_params.is_cuda and not os.environ.get("DN_TUNE_NO_WGRAD_STREAM")
         # BatchNorm backward's sums in the epilogue of the data gradient that produces the unit's activation gradient
-        self.fuse_bn_sums = not os.environ.get("DN_TUNE_NO_BN_SUMS")
+        self.fuse_bn_sums = norm == "batch" and not os.environ.get("DN_TUNE_NO_BN_SUMS")
         self.fuse_bn_sums_convt = not os.environ.get("DN_TUNE_NO_BN_SUMS_CONVT")   # ... of the transposed convolution's data gradient
         self._wgrad_stream = None
         self.two_stream_max_pixels = 20_000_000       # N*H*W above which backward stays on one stream (see _side)
@@ -195,6 +211,16 @@ class HipUNet(ParameterTree):
         for u in self.conv_units:
             w = self.tensor(u.conv + ".weight")
             b = self.tensor(u.conv + ".bias")
+            if self.norm == "group":        # nothing to fold: the statistics are the input's own
+                entry = {"bias": self._padvec(b)}
+                if u.cin == 1:
+                    kh, kw = self.kernel_size
+                    entry["wf"] = torch.zeros((kh * kw, hip.channel_pad(u.cout)), dtype=torch.float32, device=self.device)
+                    entry["wf"][:, :u.cout] = w.reshape(u.cout, kh * kw).t()
+                else:
+                    entry["w"] = self._pack(self._virtual_weight(u, w), None, hip.PACK_FWD)
+                cache[u.conv] = entry
+                continue
             gamma, beta = self.tensor(u.bn + ".weight"), self.tensor(u.bn + ".bias")
             rm, rv = self.tensor(u.bn + ".running_mean"), self.tensor(u.bn + ".running_var")
             scale = gamma / torch.sqrt(rv + BN_EPS)
@@ -336,6 +362,71 @@ class HipUNet(ParameterTree):
         hip.check(hip.lib.dn_head_1x1(cur.ref(c[0]), hip.ptr(cache["head_w"]), hip.ptr(cache["head_b"]),
                                       hip.ptr(logits), hip.ptr(probs), n, h, w, dt, hip.stream_ptr()))
 
+    def _group_norm_workspace(self, channels: int, n: int, h: int, w: int) -> torch.Tensor:
+        """The model's group-norm workspace (zeroed when allocated; the passes of one model follow each other)."""
+        ws = self._workspace()
+        need = hip.lib.dn_group_norm_workspace_bytes(n, channels, h, w, self.num_groups, self.dtype)
+        if need < 0:
+            hip.check(1)
+        if ws.get("group_norm") is None or ws["group_norm"].numel() < need:
+            ws["group_norm"] = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        return ws["group_norm"]
+
+    def _group_norm(self, u: ConvUnit, y, dst, n, h, w, arena: StepArena) -> GroupNormStats:
+        """dst = act(group_norm(y)); the statistics live in the pass's arena."""
+        flat = arena.take((GroupNormStats.floats(n, u.cout, self.num_groups),), torch.float32)
+        stats = GroupNormStats.from_flat(flat, n, u.cout, self.num_groups, self.activation)
+        group_norm_act(y, self.tensor(u.bn + ".weight").data, self.tensor(u.bn + ".bias").data, self.num_groups, GN_EPS, self.activation,
+                       out=dst, stats=stats, workspace=self._group_norm_workspace(u.cout, n, h, w))
+        return stats
+
+    @torch.no_grad()
+    def _forward_eval_chunk_group(self, x: torch.Tensor, logits: Optional[torch.Tensor], probs: Optional[torch.Tensor]):
+        """The eval forward of a ``norm="group"`` net: convolution + bias, then group norm + activation over its output in
+        place."""
+        n, _, h, w = x.shape
+        depth, f, dt, dev = self.depth, self.num_filters, self.dtype, self.device
+        c = [f * 2 ** l for l in range(depth + 1)]
+        ws = [w >> l for l in range(depth + 1)]
+        cache = self._eval_cache
+        units = {u.conv: u for u in self.conv_units}
+        A = self._arena("eval", n, h, w)
+
+        def unit(name, l, src, dst):
+            self._conv(units[name], cache[name], src, dst, n, h, ws[l], relu=0)
+            self._group_norm(units[name], dst, dst, n, h, ws[l], A)
+
+        def double(prefix, l, src, dst_buf=None, plane0=0):
+            tmp = PlaneBuffer(n, self._pp(c[l]), h, ws[l], dt, dev, arena=A)
+            unit(prefix + ".0", l, src, tmp.ref(c[l]))
+            out = dst_buf or PlaneBuffer(n, self._pp(c[l]), h, ws[l], dt, dev, arena=A)
+            unit(prefix + ".3", l, tmp.ref(c[l]), out.ref(c[l], plane0))
+            A.release(tmp.data)
+            return out
+
+        cat = [PlaneBuffer(n, 2 * self._pp(c[l]), h, ws[l], dt, dev, arena=A) for l in range(depth)]
+        cur, cur_ref = None, x
+        for l in range(depth):
+            double(f"encoders.{l}.conv.double_conv", l, cur_ref, cat[l], self._pp(c[l]))
+            if cur is not None:
+                A.release(cur.data)
+            cur = PlaneBuffer(n, self._pp(c[l]), h, ws[l + 1], dt, dev, arena=A)
+            cur_ref = cur.ref(c[l])
+            hip.check(hip.lib.dn_maxpool_1x2(cat[l].ref(c[l], self._pp(c[l])), cur_ref, n, h, ws[l + 1], dt, hip.stream_ptr()))
+        out = double("bottleneck.double_conv", depth, cur_ref)
+        A.release(cur.data)
+        cur = out
+        for i in range(depth):
+            l = depth - 1 - i
+            up = cache[f"decoders.{i}.up"]
+            hip.check(hip.lib.dn_conv_transpose_1x2(cur.ref(c[l + 1]), hip.ptr(up["w"]), hip.ptr(up["bias"]), cat[l].ref(c[l], 0), n, h,
+                                                    ws[l + 1], dt, hip.stream_ptr()))
+            A.release(cur.data)
+            cur = double(f"decoders.{i}.conv.double_conv", l, cat[l].ref(2 * self._cpad_planes(c[l]), 0))
+            A.release(cat[l].data)
+        hip.check(hip.lib.dn_head_1x1(cur.ref(c[0]), hip.ptr(cache["head_w"]), hip.ptr(cache["head_b"]), hip.ptr(logits), hip.ptr(probs), n,
+                                      h, w, dt, hip.stream_ptr()))
+
     @torch.no_grad()
     def _forward_eval_chunk_x3(self, x: torch.Tensor, logits: Optional[torch.Tensor], probs: Optional[torch.Tensor]):
         """The eval forward with hi + lo split tensors on the ``split_levels`` shallowest levels (``dn_*_x3``), plain bf16
@@ -449,7 +540,8 @@ class HipUNet(ParameterTree):
         probs = torch.empty_like(x) if want_probs else None
         for s in range(0, n, self.MAX_CHUNK):
             e = min(n, s + self.MAX_CHUNK)
-            chunk = self._forward_eval_chunk_x3 if self.split_levels else self._forward_eval_chunk
+            chunk = (self._forward_eval_chunk_x3 if self.split_levels else self._forward_eval_chunk_group if self.norm == "group"
+                     else self._forward_eval_chunk)
             chunk(x[s:e], logits[s:e] if want_logits else None, probs[s:e] if want_probs else None)
         return logits, probs
 
@@ -540,6 +632,15 @@ class HipUNet(ParameterTree):
         backward needs."""
         ws, cache, A = self._workspace(), self._train_cache, self._saved["arena"]
         y = PlaneBuffer(n, self._pp(u.cout), h, w, self.dtype, self.device, arena=A)
+        if self.norm == "group":
+            if self.sync_bn is not None:
+                raise ValueError("norm 'group' has no batch statistics to synchronise: train it without sync_bn")
+            self._conv(u, cache[u.conv], raw_x if u.cin == 1 else src, y.ref(u.cout), n, h, w, relu=0)
+            stats = self._group_norm(u, y.ref(u.cout), dst, n, h, w, A)
+            if pooled is not None:
+                hip.check(hip.lib.dn_maxpool_1x2(dst, pooled, n, h, w // 2, self.dtype, hip.stream_ptr()))
+            self._saved[u.conv] = {"y": y, "a": dst, "src": src, "stats": stats, "n": n, "h": h, "w": w}
+            return
         cp = hip.channel_pad(u.cout)
         vec = A.take((4 * cp,), torch.float32)
         mean, invstd, scale, shift = (vec[i * cp:(i + 1) * cp] for i in range(4))
@@ -720,7 +821,14 @@ class HipUNet(ParameterTree):
         ws, cache, sv, A = self._workspace(), self._train_cache, self._saved[u.conv], self._saved["arena"]
         n, h, w = sv["n"], sv["h"], sv["w"]
         kh, kw = self.kernel_size
-        if self.sync_bn is not None:
+        if self.norm == "group":
+            group_norm_act_backward(g, sv["y"].ref(u.cout), self.tensor(u.bn + ".weight").data, sv["stats"], out=g,
+                                    dgamma=self.grad(u.bn + ".weight"), dbeta=self.grad(u.bn + ".bias"),
+                                    workspace=self._group_norm_workspace(u.cout, n, h, w))
+            # a group's mean takes no single channel's offset away: the convolution's bias has a gradient here
+            hip.check(hip.lib.dn_channel_sum(g, hip.ptr(self.grad(u.conv + ".bias")), hip.ptr(ws["partial"]), n, h, w, self.dtype,
+                                             hip.stream_ptr()))
+        elif self.sync_bn is not None:
             all_reduce, world = self.sync_bn
             local = A.take((2 * hip.channel_pad(u.cout),), torch.float64)
             if sums is not None:
@@ -749,7 +857,7 @@ class HipUNet(ParameterTree):
                 hip.ptr(self.tensor(u.bn + ".weight")), hip.ptr(sv["mean"]),
                 hip.ptr(sv["invstd"]), hip.ptr(self.grad(u.bn + ".weight")), hip.ptr(self.grad(u.bn + ".bias")),
                 hip.ptr(ws["coef"]), hip.ptr(ws["partial"]), self.dtype, hip.stream_ptr()))
-        # the conv bias feeds a BatchNorm: its gradient is identically zero, the arena entry stays 0
+        # (norm "batch") the conv bias feeds a BatchNorm: its gradient is identically zero, the arena entry stays 0
         if u.cin == 1:
             hip.check(hip.lib.dn_conv_first_wgrad(hip.ptr(self._saved["x"]), g, hip.ptr(self.grad(u.conv + ".weight")),
                                                   hip.ptr(ws["partial"]), ws["partial"].numel(), n, h, w, kh, kw, self.dtype,
@@ -923,6 +1031,11 @@ class HipAdam:
         m._param_epoch += 1
         self._zeroed = True
 
+    def frozen_constants(self) -> tuple:
+        """Everything but the learning rate and the step number that a captured step has fixed."""
+        g = self.param_groups[0]
+        return (tuple(g["betas"]), g["eps"], g["weight_decay"])
+
     def zero_grad(self):
         if not self._zeroed:
             self.model.flat_grads.zero_()
@@ -934,14 +1047,13 @@ class GraphedTrainStep:
     launches for the shipped net -- captured once into a HIP graph and replayed.  At train.py's batch of 16 the step is
     otherwise bound by the host issuing those launches (trainable_unet.py:339-347 is the loop being replaced).
 
-    Batch shape, betas / eps / weight decay are frozen into the graph (``matches`` tells whether a batch fits); the
-    learning rate and the Adam step count live in device memory, so ExponentialLR keeps working.  The buffers of the
+    ``optimizer``: a ``HipAdam`` or ``HipAdamW`` of the model.  Batch shape, betas / eps / weight decay are frozen into the
+    graph (``matches`` tells whether a batch fits); the learning rate and the Adam step count live in device memory, so ExponentialLR keeps working.  The buffers of the
     step (its own ``StepArena``) stay allocated in the graph's private pool (~110 MB per bf16 profile)."""
 
-    def __init__(self, model: "HipUNet", optimizer: HipAdam, x: torch.Tensor, t: torch.Tensor):
+    def __init__(self, model: "HipUNet", optimizer, x: torch.Tensor, t: torch.Tensor):
         self.model, self.optimizer = model, optimizer
-        g = optimizer.param_groups[0]
-        self._frozen = (tuple(x.shape), tuple(g["betas"]), g["eps"], g["weight_decay"])
+        self._frozen = (tuple(x.shape), optimizer.frozen_constants())
         self.x = x.detach().clone().contiguous()
         self.t = t.detach().to(torch.int8).contiguous().clone()
         self.hyper = torch.zeros(4, dtype=torch.float32, device=model.device)
@@ -969,12 +1081,12 @@ class GraphedTrainStep:
             model._arena_override = None
         # capture executed nothing: undo the host-side bookkeeping it did
         optimizer.step_count, model._param_epoch = saved_count, saved_epoch
-        self._cache = model._train_cache                   # the images the graph writes: keep them alive
+        self._cache = model._train_cache                   # the images the graph writes: keep them alive ...
+        self._ws = dict(model._workspace())                # ... and the workspaces, which a later, larger batch replaces
         model._train_cache_version = None
 
     def matches(self, x: torch.Tensor) -> bool:
-        g = self.optimizer.param_groups[0]
-        return self._frozen == (tuple(x.shape), tuple(g["betas"]), g["eps"], g["weight_decay"])
+        return self._frozen == (tuple(x.shape), self.optimizer.frozen_constants())
 
     def __call__(self, x: torch.Tensor, t: torch.Tensor) -> torch.Tensor:
         """Runs one step on (x, t); returns a snapshot of the Dice sums vector (``HipUNet.dice_forward``)."""
