@@ -265,6 +265,64 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_param_kernel(const float2* 
   if (threadIdx.x == 0) { dbeta[c] = (float)s1; dgamma[c] = (float)s2; }
 }
 
+// The same for many partials: block (plane, chunk) adds up the rows of its chunk, all channels of the plane side by side, and
+// the plane's last block to finish adds the chunks in their order.  `counts` is zero before and after.
+int gn_param_chunks(const GnShape& s) {
+  const long rows = (long)s.N * s.nseg;
+  return (int)std::max(1L, std::min({rows / 64, 64L, 4096L / s.P}));
+}
+template <int EPR>
+__global__ __launch_bounds__(GN_THREADS) void gn_bwd_param_chunk_kernel(const float2* part, GnShape s, int chunks, unsigned* counts,
+                                                                        double2* sums, float* dgamma, float* dbeta) {
+  constexpr int ROWS = GN_THREADS / EPR;
+  __shared__ double2 red[GN_THREADS];
+  __shared__ bool last;
+  const int plane = blockIdx.x, chunk = blockIdx.y, slot = threadIdx.x % EPR, row0 = threadIdx.x / EPR;
+  const unsigned rows = (unsigned)s.N * s.nseg, per = (rows + chunks - 1) / chunks, end = min(rows, (chunk + 1) * per);
+  double2 v = make_double2(0.0, 0.0);
+  auto join = [&]() {                            // v of the threads of a slot, in a fixed order, to the threads of row 0
+    red[threadIdx.x] = v;
+    __syncthreads();
+    if (row0 == 0) {
+      v = make_double2(0.0, 0.0);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) { v.x += red[r * EPR + slot].x; v.y += red[r * EPR + slot].y; }
+    }
+    __syncthreads();
+  };
+#pragma unroll 4
+  for (unsigned r = chunk * per + row0; r < end; r += ROWS) {
+    const unsigned n = r / (unsigned)s.nseg;
+    const float2 q = part[(((long)n * s.P + plane) * s.nseg + (r - n * s.nseg)) * EPR + slot];
+    v.x += q.x;
+    v.y += q.y;
+  }
+  join();
+  if (chunks > 1) {
+    double2* mine = sums + (long)plane * chunks * EPR;
+    if (row0 == 0) {
+      mine[chunk * EPR + slot] = v;
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+    }
+    if (threadIdx.x == 0)
+      last = __hip_atomic_fetch_add(counts + plane, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)chunks - 1;
+    __syncthreads();
+    if (!last) return;
+    if (threadIdx.x == 0) __hip_atomic_store(counts + plane, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    v = make_double2(0.0, 0.0);
+#pragma unroll 4
+    for (int k = row0; k < chunks; k += ROWS) {
+      const double2 q = mine[k * EPR + slot];
+      v.x += q.x;
+      v.y += q.y;
+    }
+    join();
+  }
+  const int c = plane * EPR + slot;
+  if (row0 == 0 && c < s.C) { dbeta[c] = (float)v.x; dgamma[c] = (float)v.y; }
+}
+
 // dx may be g: a thread reads what it writes
 template <typename T, int ACT>
 __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const unsigned char* g, int g_pt, int g_p0, const unsigned char* x,
@@ -302,13 +360,631 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const unsigned
   }
 }
 
+
+// ---- one pass: the blocks of a group hold its values in registers and exchange their sums --------------------------------
+// The smallest traffic a group norm can have is one read and one write; statistics in a launch of their own cost a second
+// read.  Here a block keeps its segment in registers, publishes the segment's sums, waits for those of the other blocks of its
+// cluster -- the segments of the planes whose channels form whole groups -- and finishes from registers.
+//
+// A wait may not depend on how many blocks the chip holds or in which order it starts them: an XCD that is full of blocks which
+// wait for blocks that are to start on it would wait for ever.  Three things:
+//  * A block draws its place when it STARTS, from the counter of its shard, and consecutive places of a shard are a cluster:
+//    whatever the order, at most one cluster per shard is incomplete, and only its blocks wait for blocks to come.
+//  * There are as few shards as that the blocks of all incomplete clusters (GNF_WAITING) do not fill the slots of a single XCD,
+//    to which the blocks not yet started may all have been dealt.  (One counter alone costs 60 ns per block, one after the
+//    other: 418 us instead of 190 for 256 x 32 x 6 x 4096 bf16.  Clusters kept within an XCD: 216 us.)
+//  * A wait is bounded all the same.  A block that gives up has published its own sums; it puts its place on a list and exits,
+//    which frees its slot on the chip.  The launch's last block finds all sums published and does the listed segments over.
+// So every wait ends and every segment is written, with the same bits, whatever else runs on the GPU.
+//
+// A published word carries the launch's epoch beside its 32-bit value, so no fence and no clearing is needed: words of earlier
+// launches have other epochs.  The launch's last block counts the epoch up; counters return to zero.
+constexpr int GNF_THREADS = 512;
+constexpr int GNF_WAVES = GNF_THREADS / 64;
+constexpr int GNF_MAX_K = 64;                    // blocks of a cluster
+constexpr int GNF_MAX_CELLS = 1024;              // published cells of a cluster
+constexpr int GNF_MAX_BLOCKS = 16384;            // blocks of a launch: more images take more launches
+constexpr int GNF_POLLS = 4096;                  // looks at a word before a block gives up: about 0.6 ms
+constexpr int GNF_SHARDS = 16;                   // counters of places at most
+constexpr int GNF_WAITING = 80;                  // blocks of incomplete clusters at most: an XCD holds 96 (32 CUs x 3 blocks of 80 registers)
+constexpr int GNF_LINE = 32;                     // counters 128 bytes apart: epoch, finished shards, listed, then two per shard
+constexpr long GNF_CTRL_BYTES = (3 + 2 * GNF_SHARDS) * GNF_LINE * 4L, GNF_DEPART_BYTES = GNF_MAX_BLOCKS * 4L;
+constexpr long GNF_LIST0 = GNF_CTRL_BYTES + GNF_DEPART_BYTES;
+constexpr long GNF_SLOT0 = GNF_LIST0 + GNF_MAX_BLOCKS * 8L;
+constexpr long GNF_END = GNF_SLOT0 + GNF_MAX_BLOCKS * 16L * 16;      // the three-launch form's partials lie behind: no word of theirs
+                                                                     // can be taken for a published one
+// Division of a small number by one that the host knows: one multiplication (exact while number * divisor < 2^32; divisor 1 has
+// mul 0).  A division by a runtime value is some 20 dependent instructions, and a dozen of them lie on a block's critical path.
+struct GnDiv {
+  unsigned d, mul;
+};
+__device__ __forceinline__ int gn_div(const GnDiv& v, int n) { return v.mul ? (int)__umulhi((unsigned)n, v.mul) : n; }
+__device__ __forceinline__ int gn_mod(const GnDiv& v, int n) { return n - gn_div(v, n) * (int)v.d; }
+GnDiv gn_divisor(long d) { return GnDiv{(unsigned)d, d > 1 ? (unsigned)((1ULL << 32) / (unsigned long)d) + 1 : 0}; }
+
+struct GnFused {
+  GnShape s;
+  int m;                   // channels of a cell: gcd(channels per group, channels per record)
+  int ncell;               // cells of a plane
+  int ps, nsets;           // planes of a cluster, clusters of an image
+  int shards, polls;
+  int image0, images;      // this launch's
+  GnDiv d_most, d_shards, d_nsets, d_nseg, d_cpg, d_m;
+  double inv_total;        // 1 / values of a group
+  unsigned* ctrl;          // counters, GNF_LINE words apart
+  unsigned* depart;        // per cluster: blocks that wait no longer
+  unsigned long long* list;      // places that were given up, with the epoch
+  unsigned long long* slot;
+};
+
+// The packed pieces stay in registers and are unpacked anew by each pass over them: kept unpacked, they would fill twice the
+// registers and halve the blocks that a CU holds.
+template <int R> __device__ __forceinline__ void gnf_keep_packed(uint4 (&v)[R]) {
+#pragma unroll
+  for (int k = 0; k < R; ++k) asm volatile("" : "+v"(v[k].x), "+v"(v[k].y), "+v"(v[k].z), "+v"(v[k].w));
+}
+
+// Four channels of a piece: the passes below take a bf16 piece in two halves, so that the constants of four channels and not of
+// eight are held at a time.
+template <typename T> __device__ __forceinline__ void gnf_unpack4(const uint4& v, int h, float* f);
+template <> __device__ __forceinline__ void gnf_unpack4<float>(const uint4& v, int, float* f) { Piece<float>::unpack(v, f); }
+template <> __device__ __forceinline__ void gnf_unpack4<__bf16>(const uint4& v, int h, float* f) {
+  const unsigned a = h ? v.z : v.x, b = h ? v.w : v.y;
+  f[0] = __uint_as_float(a << 16); f[1] = __uint_as_float(a & 0xffff0000u);
+  f[2] = __uint_as_float(b << 16); f[3] = __uint_as_float(b & 0xffff0000u);
+}
+template <typename T> __device__ __forceinline__ void gnf_pack4(uint4& v, int h, const float* f);
+template <> __device__ __forceinline__ void gnf_pack4<float>(uint4& v, int, const float* f) { v = Piece<float>::pack(f); }
+template <> __device__ __forceinline__ void gnf_pack4<__bf16>(uint4& v, int h, const float* f) {
+  typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;           // a pair in one conversion
+  unsigned lo = __builtin_bit_cast(unsigned, (bf16x2_t){(__bf16)f[0], (__bf16)f[1]});
+  unsigned hi = __builtin_bit_cast(unsigned, (bf16x2_t){(__bf16)f[2], (__bf16)f[3]});
+  asm volatile("" : "+v"(lo), "+v"(hi));                                 // packed here and not where it is stored
+  if (h) { v.z = lo; v.w = hi; } else { v.x = lo; v.y = hi; }
+}
+
+struct GnPlace { int plane, seg, lo, hi, k, set, shard; long n, cluster0, cluster; unsigned place, tag; bool alone; };
+
+__device__ __forceinline__ unsigned gnf_count(unsigned* p) {
+  return __hip_atomic_fetch_add(p, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void gnf_reset(unsigned* p) { __hip_atomic_store(p, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ int gnf_shard_clusters(const GnFused& f, int shard) {
+  return gn_div(f.d_shards, f.images * f.nsets - shard + f.shards - 1);
+}
+
+// What place `b` of shard u.shard is.  Clusters are laid out as if all had f.ps planes: plane >= P, as a cluster past the
+// last, is a block with nothing to do.
+__device__ __forceinline__ void gnf_locate(const GnFused& f, GnPlace& u, unsigned b) {
+  const GnShape& s = f.s;
+  u.place = b;
+  const int nth = gn_div(f.d_most, (int)b), member = (int)b - nth * (int)f.d_most.d, cluster = u.shard + f.shards * nth;
+  const int image = gn_div(f.d_nsets, cluster);
+  u.cluster = cluster;
+  u.set = cluster - image * f.nsets;
+  const int plane = gn_div(f.d_nseg, member);
+  u.plane = u.set * f.ps + plane;
+  u.seg = member - plane * s.nseg;
+  u.n = (long)f.image0 + image;
+  u.lo = u.seg * s.seg_len;
+  u.hi = min(s.npieces, u.lo + s.seg_len);
+  u.k = min(f.ps, s.P - u.set * f.ps) * s.nseg;
+  u.cluster0 = u.cluster * (long)f.d_most.d;     // the cluster's first block in the slots
+}
+// This block's place (LDS broadcast; one barrier); false: nothing to do.
+__device__ __forceinline__ bool gnf_place(const GnFused& f, unsigned* lds2, GnPlace& u) {
+  u.alone = f.d_most.d == 1;                           // every cluster of the launch is one block: nothing is exchanged
+  u.shard = gn_mod(f.d_shards, gn_div(f.d_most, (int)blockIdx.x));
+  if (threadIdx.x == 0) {
+    unsigned place = (unsigned)gn_div(f.d_shards, (int)blockIdx.x), epoch = 0;
+    if (!u.alone) {
+      unsigned* next = f.ctrl + (3 + 2 * u.shard) * GNF_LINE;
+      place = gnf_count(next);
+      if (place == (unsigned)gn_div(f.d_shards, (int)gridDim.x) - 1) gnf_reset(next);                // the shard's last block to start
+      epoch = __hip_atomic_load(f.ctrl, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    lds2[0] = place;
+    lds2[1] = epoch;
+    lds2[2] = 0;
+  }
+  __syncthreads();
+  u.tag = (unsigned)__builtin_amdgcn_readfirstlane(lds2[1]) % 0xFFFFFFFFu + 1;         // never 0, what the workspace is filled with at first
+  gnf_locate(f, u, __builtin_amdgcn_readfirstlane(lds2[0]));                           // scalar from here on
+  return u.cluster < (long)f.images * f.nsets && u.plane < f.s.P;
+}
+
+// Sums over the wave's 32 lanes of equal record half, of four channels at a time (h: which four of the thread's half record):
+// two halving steps leave a channel to a lane, three more add the lanes up.  Lanes 0..7 put them into the wave's row of `red`.
+template <int M> __device__ __forceinline__ float gnf_xor(float v) {          // the value of lane ^ M
+  if constexpr (M < 32) return __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(v), M << 10 | 0x1F));
+  else return __shfl_xor(v, M);
+}
+template <int WIDTH, int M> __device__ __forceinline__ void gnf_halve(float* acc) {     // 2 * WIDTH values -> WIDTH
+  const bool upper = threadIdx.x & M;
+#pragma unroll
+  for (int j = 0; j < WIDTH; ++j) {
+    const float give = upper ? acc[j] : acc[j + WIDTH];
+    const float keep = upper ? acc[j + WIDTH] : acc[j];
+    acc[j] = keep + gnf_xor<M>(give);
+  }
+  if constexpr (WIDTH > 1) gnf_halve<WIDTH / 2, M * 2>(acc);
+}
+template <int PN> __device__ __forceinline__ void gnf_wave_sums(float (&acc)[4], int h, float* red) {
+  gnf_halve<2, 2>(acc);
+  float v = acc[0];
+  v += gnf_xor<8>(v);
+  v += gnf_xor<16>(v);
+  v += gnf_xor<32>(v);
+  const int lane = threadIdx.x & 63;
+  if (lane < 8) red[(threadIdx.x >> 6) * 2 * PN + (lane & 1) * PN + 4 * h + (lane & 2) + (lane >> 2)] = v;
+}
+// After a barrier: the block's sum of channel lane % EPR, in every wave.
+template <int PN> __device__ __forceinline__ float gnf_block_sum(const float* red) {
+  constexpr int EPR = 2 * PN, ROWS = 64 / EPR;
+  const int lane = threadIdx.x & 63;
+  float t = 0.f;
+#pragma unroll
+  for (int w = 0; w < GNF_WAVES; w += ROWS) t += red[w * EPR + lane];          // waves w + lane / EPR
+  if constexpr (EPR == 8) t += gnf_xor<8>(t);
+  t += gnf_xor<16>(t);
+  t += gnf_xor<32>(t);
+  return t;
+}
+
+__device__ __forceinline__ void gnf_publish(const GnFused& f, const GnPlace& u, int cell, float a, float b) {
+  unsigned long long* p = f.slot + ((u.cluster0 + (long)(u.plane - u.set * f.ps) * f.s.nseg + u.seg) * f.ncell + cell) * 2;
+  const unsigned long long tag = (unsigned long long)u.tag << 32;
+  __hip_atomic_store(p, tag | __float_as_uint(a), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __hip_atomic_store(p + 1, tag | __float_as_uint(b), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// All cells of the cluster into LDS (words 2 * cell, 2 * cell + 1); false: given up, the place is on the list.  Ends with a
+// barrier.  *before (thread GNF_COUNTER): blocks of the cluster that waited no longer before this one; the count is under way when
+// the call returns, its first use waits for it.  *missing is 0 at the call.
+constexpr unsigned GNF_COUNTER = 64;             // not thread 0, which has work to do next
+__device__ __forceinline__ bool gnf_collect(const GnFused& f, const GnPlace& u, float* cells, unsigned* missing, unsigned* before) {
+  const int words = u.k * f.ncell * 2;
+  const unsigned long long* p = f.slot + u.cluster0 * f.ncell * 2;
+  for (int w = threadIdx.x; w < words; w += GNF_THREADS) {
+    unsigned long long v = __hip_atomic_load(p + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int tries = 0; (unsigned)(v >> 32) != u.tag && tries < f.polls; ++tries) {
+      __builtin_amdgcn_s_sleep(1);
+      v = __hip_atomic_load(p + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if ((unsigned)(v >> 32) != u.tag) *missing = 1;
+    cells[w] = __uint_as_float((unsigned)v);
+  }
+  __syncthreads();
+  const bool given_up = __builtin_amdgcn_readfirstlane(*missing) != 0;
+  if (threadIdx.x == GNF_COUNTER) {
+    if (given_up) {
+      const unsigned at = gnf_count(f.ctrl + 2 * GNF_LINE);
+      if (at < GNF_MAX_BLOCKS)
+        __hip_atomic_store(f.list + at, (unsigned long long)u.tag << 32 | (unsigned)u.shard << 24 | u.place, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");                                         // the list before the departure
+    }
+    *before = gnf_count(f.depart + u.cluster);
+  }
+  return !given_up;
+}
+// The launch's last block to wait: everything is there, with or without patience.
+__device__ __forceinline__ void gnf_collect_again(const GnFused& f, const GnPlace& u, float* cells) {
+  const unsigned long long* p = f.slot + u.cluster0 * f.ncell * 2;
+  for (int w = threadIdx.x; w < u.k * f.ncell * 2; w += GNF_THREADS)
+    cells[w] = __uint_as_float((unsigned)__hip_atomic_load(p + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  __syncthreads();
+}
+// Whether this block is the launch's last to wait (thread GNF_COUNTER; the answer is for after the next barrier).
+__device__ __forceinline__ void gnf_last(const GnFused& f, const GnPlace& u, unsigned before, unsigned* last) {
+  if (u.alone || threadIdx.x != GNF_COUNTER) return;
+  *last = 0;
+  if (before != (unsigned)u.k - 1) return;
+  gnf_reset(f.depart + u.cluster);                                                             // the cluster's last
+  unsigned* finished = f.ctrl + (4 + 2 * u.shard) * GNF_LINE;
+  if (gnf_count(finished) != (unsigned)gnf_shard_clusters(f, u.shard) - 1) return;
+  gnf_reset(finished);                                                                         // the shard's last
+  if (gnf_count(f.ctrl + GNF_LINE) != (unsigned)min(f.shards, f.images * f.nsets) - 1) return;
+  gnf_reset(f.ctrl + GNF_LINE);                                                                // the launch's last
+  *last = 1;
+}
+// The launch's last block: the next listed place into `u`; false: none is left, the epoch is counted up.  (One barrier.)
+__device__ __forceinline__ bool gnf_next_listed(const GnFused& f, GnPlace& u, unsigned* at, unsigned* lds2) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    lds2[0] = 0xFFFFFFFFu;
+    if (*at == 0) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    const unsigned listed = __hip_atomic_load(f.ctrl + 2 * GNF_LINE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (*at < listed && *at < GNF_MAX_BLOCKS) {
+      unsigned long long v = 0;
+      for (int tries = 0; (unsigned)(v >> 32) != u.tag && tries < 1 << 22; ++tries)
+        v = __hip_atomic_load(f.list + *at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      lds2[0] = (unsigned)v;
+    } else {
+      gnf_reset(f.ctrl + 2 * GNF_LINE);
+      gnf_count(f.ctrl);
+    }
+  }
+  __syncthreads();
+  const unsigned v = __builtin_amdgcn_readfirstlane(lds2[0]);
+  if (v == 0xFFFFFFFFu) return false;
+  ++*at;
+  u.shard = (int)(v >> 24);
+  gnf_locate(f, u, v & 0xFFFFFFu);
+  return u.cluster < (long)f.images * f.nsets && u.plane < f.s.P;
+}
+
+__device__ __forceinline__ void gnf_wave_sum64(double& a, double& b) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) {
+    a += __shfl_xor(a, m);
+    b += __shfl_xor(b, m);
+  }
+}
+
+// the cell (index in LDS) and segment of a group's i-th contribution
+__device__ __forceinline__ int gnf_cell(const GnFused& f, const GnPlace& u, int epr, int g, int i, int* seg) {
+  const int j = gn_div(f.d_nseg, i);
+  *seg = i - j * f.s.nseg;
+  const int c = g * f.s.cpg + j * f.m;
+  return ((c / epr - u.set * f.ps) * f.s.nseg + *seg) * f.ncell + gn_div(f.d_m, c % epr);
+}
+
+template <int EPR> struct GnfShared {
+  unsigned place[3], last;                       // {place, epoch, missing}
+  float red[2][GNF_WAVES * EPR], cells[GNF_MAX_CELLS * 2], gstat[EPR][2], chan[EPR][7];
+};
+
+template <int R> __device__ __forceinline__ void gnf_load(uint4 (&v)[R], const void* base, int pt, int p0, const GnShape& s, const GnPlace& u) {
+  const unsigned char* b = (const unsigned char*)base + ((u.n * pt + p0 + u.plane) * (long)s.npieces + u.lo) * 16;
+  const int len = u.hi - u.lo;
+#pragma unroll
+  for (int k = 0; k < R; ++k) {
+    const int i = (int)threadIdx.x + k * GNF_THREADS;
+    v[k] = i < len ? *(const uint4*)(b + (unsigned)i * 16u) : make_uint4(0, 0, 0, 0);
+  }
+}
+
+struct GnForward {
+  const void* x;
+  void* a;
+  int x_pt, x_p0, a_pt, a_p0;
+  const float *gamma, *beta;
+  float eps;
+  float *mean, *rstd, *scale, *shift;
+};
+// From the cluster's cells in LDS to the statistics of this plane's groups, scale and shift of its channels (sh.chan).  Between
+// two barriers.  `leave()` runs on the way.
+template <int EPR, typename F>
+__device__ __forceinline__ void gnf_scales(const GnFused& f, const GnForward& o, const GnPlace& u, GnfShared<EPR>& sh, F leave) {
+  const GnShape& s = f.s;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // the groups of this plane's channels, a wave each: M2 = sum M2_i + sum n_i (mean_i - mean)^2
+  const int c_lo = u.plane * EPR, c_hi = min(s.C, c_lo + EPR);
+  const int g_lo = gn_div(f.d_cpg, c_lo), g_hi = gn_div(f.d_cpg, c_hi - 1);
+  const int parts = gn_div(f.d_m, s.cpg) * s.nseg;
+  for (int g = g_lo + wave; g <= g_hi; g += GNF_WAVES) {
+    // around the first part's mean: M2 = sum (M2_i + n_i d_i^2) - (sum n_i d_i)^2 / n, d_i = mean_i - pivot, in fp64
+    int seg;
+    const double pivot = (double)sh.cells[2 * gnf_cell(f, u, EPR, g, 0, &seg)];
+    double s1 = 0.0, s2 = 0.0;
+    for (int i = lane; i < parts; i += 64) {
+      const int at = gnf_cell(f, u, EPR, g, i, &seg);
+      const double d = (double)sh.cells[2 * at] - pivot;
+      const double nd = (double)(f.m * (min(s.npieces, (seg + 1) * s.seg_len) - seg * s.seg_len) / 2) * d;
+      s1 += nd;
+      s2 += (double)sh.cells[2 * at + 1] + nd * d;
+    }
+    gnf_wave_sum64(s1, s2);
+    const double shift = s1 * f.inv_total;
+    const float mean32 = (float)(pivot + shift);
+    const float var = (float)((s2 - s1 * shift) * f.inv_total + (double)o.eps);
+    float rstd = __builtin_amdgcn_rsqf(var);
+    rstd = fmaf(rstd * 0.5f, fmaf(-var * rstd, rstd, 1.f), rstd);                // one Newton step
+    if (lane == 0) {
+      sh.gstat[g - g_lo][0] = mean32;
+      sh.gstat[g - g_lo][1] = rstd;
+      if (u.seg == 0 && g * s.cpg >= c_lo) { o.mean[u.n * s.G + g] = mean32; o.rstd[u.n * s.G + g] = rstd; }
+    }
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < EPR) {
+    const int c = c_lo + threadIdx.x;
+    float c_scale = 0.f, c_shift = 0.f;
+    if (c < s.C) {
+      const int g = gn_div(f.d_cpg, c) - g_lo;
+      c_scale = o.gamma[c] * sh.gstat[g][1];
+      c_shift = fmaf(-sh.gstat[g][0], c_scale, o.beta[c]);
+    }
+    sh.chan[threadIdx.x][0] = c_scale;
+    sh.chan[threadIdx.x][1] = c_shift;
+    if (u.seg == 0) { o.scale[u.n * s.cpad + c] = c_scale; o.shift[u.n * s.cpad + c] = c_shift; }
+  } else if (u.seg == 0 && u.plane == s.P - 1) {                               // vector entries past the last plane
+    for (int c = s.P * EPR + (int)threadIdx.x - EPR; c < s.cpad; c += GNF_THREADS - EPR) { o.scale[u.n * s.cpad + c] = 0.f; o.shift[u.n * s.cpad + c] = 0.f; }
+  }
+  leave();
+  __syncthreads();
+}
+// Pieces first, first + GNF_THREADS, ... of the segment: v = act(v * scale + shift), stored.
+template <typename T, int ACT, int R>
+__device__ __forceinline__ void gnf_apply(const GnForward& o, const GnShape& s, const GnPlace& u, uint4 (&v)[R], int first,
+                                          const GnfShared<RecTraits<T>::EPR>& sh) {
+  constexpr int PN = Piece<T>::N;
+  const int pc = threadIdx.x & 1, len = u.hi - u.lo;
+  unsigned char* ab = (unsigned char*)o.a + ((u.n * o.a_pt + o.a_p0 + u.plane) * (long)s.npieces + u.lo) * 16;
+#pragma unroll
+  for (int h = 0; h < PN / 4; ++h) {
+    float sc[4], sf[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { sc[j] = sh.chan[pc * PN + 4 * h + j][0]; sf[j] = sh.chan[pc * PN + 4 * h + j][1]; }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      float t[4];
+      gnf_unpack4<T>(v[k], h, t);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t[j] = gn_act<ACT>(fmaf(t[j], sc[j], sf[j]));
+      gnf_pack4<T>(v[k], h, t);
+      const int i = first + k * GNF_THREADS;
+      if (h == PN / 4 - 1 && i < len) *(uint4*)(ab + (unsigned)i * 16u) = v[k];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+template <typename T, int ACT, int R>
+__global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_kernel(GnFused f, GnForward o) {
+  constexpr int PN = Piece<T>::N, EPR = RecTraits<T>::EPR;
+  __shared__ GnfShared<EPR> sh;
+  GnPlace u;
+  if (!gnf_place(f, sh.place, u)) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pc = threadIdx.x & 1, len = u.hi - u.lo;
+  uint4 v[R];
+  gnf_load<R>(v, o.x, o.x_pt, o.x_p0, f.s, u);
+#pragma unroll
+  for (int h = 0; h < PN / 4; ++h) {
+    float acc[4] = {};
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      float t[4];
+      gnf_unpack4<T>(v[k], h, t);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] += t[j];
+      __builtin_amdgcn_sched_barrier(0);                   // piece after piece: interleaved, they would need twice the registers
+    }
+    gnf_wave_sums<PN>(acc, h, sh.red[0]);
+  }
+  __syncthreads();
+  float sum = gnf_block_sum<PN>(sh.red[0]);
+  for (int x2 = 1; x2 < f.m; x2 <<= 1) sum += __shfl_xor(sum, x2);             // over the cell's channels
+  const float cmean = sum / (float)(f.m * (len / 2));
+  gnf_keep_packed<R>(v);
+#pragma unroll
+  for (int h = 0; h < PN / 4; ++h) {
+    float mu[4], acc[4] = {};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mu[j] = __shfl(cmean, pc * PN + 4 * h + j);
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      if ((int)threadIdx.x + k * GNF_THREADS < len) {
+        float t[4];
+        gnf_unpack4<T>(v[k], h, t);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = fmaf(t[j] - mu[j], t[j] - mu[j], acc[j]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    gnf_wave_sums<PN>(acc, h, sh.red[1]);
+  }
+  gnf_keep_packed<R>(v);
+  __syncthreads();
+  float m2 = gnf_block_sum<PN>(sh.red[1]);
+  for (int x2 = 1; x2 < f.m; x2 <<= 1) m2 += __shfl_xor(m2, x2);
+  const bool owner = wave == 0 && lane < EPR && gn_mod(f.d_m, lane) == 0;
+  bool got = true;
+  unsigned before = 0;
+  if (!u.alone) {
+    if (owner) gnf_publish(f, u, gn_div(f.d_m, lane), cmean, m2);
+    got = gnf_collect(f, u, sh.cells, &sh.place[2], &before);
+  } else {
+    if (owner) { sh.cells[2 * (gn_div(f.d_m, lane))] = cmean; sh.cells[2 * (gn_div(f.d_m, lane)) + 1] = m2; }
+    __syncthreads();
+  }
+  if (got) {
+    gnf_scales<EPR>(f, o, u, sh, [&] { gnf_last(f, u, before, &sh.last); });
+    gnf_apply<T, ACT, R>(o, f.s, u, v, threadIdx.x, sh);
+  } else {
+    gnf_last(f, u, before, &sh.last);
+    __syncthreads();
+  }
+  if (u.alone || !sh.last) return;
+  for (unsigned listed = 0; gnf_next_listed(f, u, &listed, sh.place);) {       // the launch's last block: what others gave up
+    gnf_collect_again(f, u, sh.cells);
+    gnf_scales<EPR>(f, o, u, sh, [] {});
+    const unsigned char* xb = (const unsigned char*)o.x + ((u.n * o.x_pt + o.x_p0 + u.plane) * (long)f.s.npieces + u.lo) * 16;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < u.hi - u.lo; i += GNF_THREADS) {
+      uint4 one[1] = {*(const uint4*)(xb + (unsigned)i * 16u)};
+      gnf_apply<T, ACT, 1>(o, f.s, u, one, i, sh);
+    }
+  }
+}
+
+// backward: part[block][channel] = (sum dz, sum dz * xhat) for the parameter gradients, group sums as above
+struct GnBackward {
+  const void *g, *x;
+  void* dx;
+  int g_pt, g_p0, x_pt, x_p0, d_pt, d_p0;
+  const float *gamma, *mean, *rstd, *scale, *shift;
+  float2* part;
+};
+template <int EPR> __device__ __forceinline__ void gnf_channels(const GnFused& f, const GnBackward& o, const GnPlace& u, GnfShared<EPR>& sh) {
+  const GnShape& s = f.s;
+  if ((int)threadIdx.x < EPR) {
+    const int c = u.plane * EPR + threadIdx.x;
+    const bool in = c < s.C;
+    float* q = sh.chan[threadIdx.x];
+    q[0] = o.scale[u.n * s.cpad + c];
+    q[1] = o.shift[u.n * s.cpad + c];
+    q[2] = in ? o.mean[u.n * s.G + gn_div(f.d_cpg, c)] : 0.f;
+    q[3] = in ? o.rstd[u.n * s.G + gn_div(f.d_cpg, c)] : 0.f;
+    q[4] = in ? o.gamma[c] : 0.f;
+  }
+  __syncthreads();
+}
+// From the cluster's cells in LDS to the constants of dx (sh.chan).  Between two barriers; `leave()` runs on the way.
+template <int EPR, typename F>
+__device__ __forceinline__ void gnf_scales_bwd(const GnFused& f, const GnPlace& u, GnfShared<EPR>& sh, F leave) {
+  const GnShape& s = f.s;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c_lo = u.plane * EPR, c_hi = min(s.C, c_lo + EPR);
+  const int g_lo = gn_div(f.d_cpg, c_lo), g_hi = gn_div(f.d_cpg, c_hi - 1);
+  const int parts = gn_div(f.d_m, s.cpg) * s.nseg;
+  for (int gi = g_lo + wave; gi <= g_hi; gi += GNF_WAVES) {
+    double p1 = 0.0, p2 = 0.0;
+    for (int i = lane; i < parts; i += 64) {
+      int seg;
+      const int at = gnf_cell(f, u, EPR, gi, i, &seg);
+      p1 += (double)sh.cells[2 * at];
+      p2 += (double)sh.cells[2 * at + 1];
+    }
+    gnf_wave_sum64(p1, p2);
+    if (lane == 0) { sh.gstat[gi - g_lo][0] = (float)(p1 * f.inv_total); sh.gstat[gi - g_lo][1] = (float)(p2 * f.inv_total); }
+  }
+  __syncthreads();
+  if ((int)threadIdx.x < EPR) {
+    const int c = c_lo + threadIdx.x;
+    const bool in = c < s.C;
+    // dx = rstd (gamma dz - c1 - (x - mean) rstd c2) = k4 dz + (k6 (x - mean) + k5)
+    const float r = sh.chan[threadIdx.x][3];
+    sh.chan[threadIdx.x][4] *= r;
+    sh.chan[threadIdx.x][5] = in ? -r * sh.gstat[gn_div(f.d_cpg, c) - g_lo][0] : 0.f;
+    sh.chan[threadIdx.x][6] = in ? -r * r * sh.gstat[gn_div(f.d_cpg, c) - g_lo][1] : 0.f;
+  }
+  leave();
+  __syncthreads();
+}
+// Pieces first, first + GNF_THREADS, ... of the segment: dx, stored.  MASKED: vg holds dz already (ReLU).
+template <typename T, int ACT, int R, bool MASKED>
+__device__ __forceinline__ void gnf_apply_bwd(const GnBackward& o, const GnShape& s, const GnPlace& u, uint4 (&vg)[R], uint4 (&vx)[R],
+                                              int first, const GnfShared<RecTraits<T>::EPR>& sh) {
+  constexpr int PN = Piece<T>::N;
+  const int pc = threadIdx.x & 1, len = u.hi - u.lo;
+  unsigned char* db = (unsigned char*)o.dx + ((u.n * o.d_pt + o.d_p0 + u.plane) * (long)s.npieces + u.lo) * 16;
+#pragma unroll
+  for (int h = 0; h < PN / 4; ++h) {
+    __builtin_amdgcn_sched_barrier(0);
+    float sc[4], sf[4], mu[4], k4[4], k5[4], k6[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float* q = sh.chan[pc * PN + 4 * h + j];
+      sc[j] = q[0]; sf[j] = q[1]; mu[j] = q[2]; k4[j] = q[4]; k5[j] = q[5]; k6[j] = q[6];
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      float fg[4], fx[4];
+      gnf_unpack4<T>(vg[k], h, fg);
+      gnf_unpack4<T>(vx[k], h, fx);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float dz = ACT == DN_ACT_SILU || !MASKED ? gn_act_grad<ACT>(fmaf(fx[j], sc[j], sf[j]), fg[j]) : fg[j];
+        fg[j] = fmaf(k4[j], dz, fmaf(k6[j], fx[j] - mu[j], k5[j]));
+      }
+      gnf_pack4<T>(vg[k], h, fg);
+      const int i = first + k * GNF_THREADS;
+      if (h == PN / 4 - 1 && i < len) *(uint4*)(db + (unsigned)i * 16u) = vg[k];
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+
+template <typename T, int ACT, int R>
+__global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_bwd_kernel(GnFused f, GnBackward o) {
+  constexpr int PN = Piece<T>::N, EPR = RecTraits<T>::EPR;
+  __shared__ GnfShared<EPR> sh;
+  const GnShape& s = f.s;
+  GnPlace u;
+  if (!gnf_place(f, sh.place, u)) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pc = threadIdx.x & 1;
+  uint4 vg[R], vx[R];
+  gnf_load<R>(vg, o.g, o.g_pt, o.g_p0, s, u);
+  gnf_load<R>(vx, o.x, o.x_pt, o.x_p0, s, u);
+  gnf_channels<EPR>(f, o, u, sh);
+#pragma unroll
+  for (int h = 0; h < PN / 4; ++h) {
+    __builtin_amdgcn_sched_barrier(0);
+    float sc[4], sf[4], mu[4], a1[4] = {}, a2[4] = {};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float* q = sh.chan[pc * PN + 4 * h + j];
+      sc[j] = q[0]; sf[j] = q[1]; mu[j] = q[2];
+    }
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+      float fg[4], fx[4];
+      gnf_unpack4<T>(vg[k], h, fg);
+      gnf_unpack4<T>(vx[k], h, fx);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float dz = gn_act_grad<ACT>(fmaf(fx[j], sc[j], sf[j]), fg[j]);   // 0 past the segment's end: fg is
+        a1[j] += dz;
+        a2[j] = fmaf(dz, fx[j] - mu[j], a2[j]);                                // times rstd below
+        fg[j] = dz;
+        asm volatile("" : "+v"(a1[j]), "+v"(a2[j]));                           // both here: one put off would keep dz and x alive
+      }
+      if constexpr (ACT == DN_ACT_RELU) gnf_pack4<T>(vg[k], h, fg);            // g or 0: dz fits where g was
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    gnf_wave_sums<PN>(a1, h, sh.red[0]);
+    gnf_wave_sums<PN>(a2, h, sh.red[1]);
+  }
+  gnf_keep_packed<R>(vg);
+  gnf_keep_packed<R>(vx);
+  __syncthreads();
+  float s1 = gnf_block_sum<PN>(sh.red[0]), s2 = gnf_block_sum<PN>(sh.red[1]);
+  const int cl = lane % EPR;
+  s2 *= sh.chan[cl][3];
+  if (wave == 0 && lane < EPR) o.part[((u.n * s.P + u.plane) * s.nseg + u.seg) * EPR + lane] = make_float2(s1, s2);
+  s1 *= sh.chan[cl][4];
+  s2 *= sh.chan[cl][4];
+  for (int x2 = 1; x2 < f.m; x2 <<= 1) { s1 += __shfl_xor(s1, x2); s2 += __shfl_xor(s2, x2); }
+  const bool owner = wave == 0 && lane < EPR && gn_mod(f.d_m, lane) == 0;
+  bool got = true;
+  unsigned before = 0;
+  if (!u.alone) {
+    if (owner) gnf_publish(f, u, gn_div(f.d_m, lane), s1, s2);
+    got = gnf_collect(f, u, sh.cells, &sh.place[2], &before);
+  } else {
+    if (owner) { sh.cells[2 * (gn_div(f.d_m, lane))] = s1; sh.cells[2 * (gn_div(f.d_m, lane)) + 1] = s2; }
+    __syncthreads();
+  }
+  if (got) {
+    gnf_scales_bwd<EPR>(f, u, sh, [&] { gnf_last(f, u, before, &sh.last); });
+    gnf_apply_bwd<T, ACT, R, true>(o, s, u, vg, vx, threadIdx.x, sh);
+  } else {
+    gnf_last(f, u, before, &sh.last);
+    __syncthreads();
+  }
+  if (u.alone || !sh.last) return;
+  for (unsigned listed = 0; gnf_next_listed(f, u, &listed, sh.place);) {       // the launch's last block: what others gave up
+    gnf_channels<EPR>(f, o, u, sh);
+    gnf_collect_again(f, u, sh.cells);
+    gnf_scales_bwd<EPR>(f, u, sh, [] {});
+    const unsigned char* gb = (const unsigned char*)o.g + ((u.n * o.g_pt + o.g_p0 + u.plane) * (long)s.npieces + u.lo) * 16;
+    const unsigned char* xb = (const unsigned char*)o.x + ((u.n * o.x_pt + o.x_p0 + u.plane) * (long)s.npieces + u.lo) * 16;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < u.hi - u.lo; i += GNF_THREADS) {
+      uint4 one_g[1] = {*(const uint4*)(gb + (unsigned)i * 16u)}, one_x[1] = {*(const uint4*)(xb + (unsigned)i * 16u)};
+      gnf_apply_bwd<T, ACT, 1, false>(o, s, u, one_g, one_x, i, sh);
+    }
+  }
+}
+
 int gn_shape(const char* name, dn_tensor x, int N, int H, int W, int groups, int dtype, GnShape* out) {
   DN_CHECK_ARG(dtype == DN_F32 || dtype == DN_BF16, "%s: bad dtype %d", name, dtype);
   DN_CHECK_ARG(N >= 0 && H >= 1 && W >= 1 && (long)H * W <= (1L << 25), "%s: bad size N=%d H=%d W=%d (H * W <= 2^25)", name, N, H, W);
   DN_CHECK_ARG(x.channels >= 1 && groups >= 1 && x.channels % groups == 0, "%s: %d channels do not divide into %d groups", name, x.channels,
                groups);
   GnShape s;
-  const int epr = dtype == DN_BF16 ? 16 : 8;
   s.N = N; s.C = x.channels; s.G = groups; s.P = dn_planes(x.channels, dtype);
   s.cpg = x.channels / groups; s.cpad = dn_channel_pad(x.channels);
   s.npieces = 2 * H * W;
@@ -316,7 +992,6 @@ int gn_shape(const char* name, dn_tensor x, int N, int H, int W, int groups, int
   s.seg_len = ((s.npieces / 2 + s.nseg - 1) / s.nseg) * 2;
   s.nseg = (s.npieces + s.seg_len - 1) / s.seg_len;
   DN_CHECK_ARG((long)N * s.P * s.nseg < (1L << 31) && (long)N * s.G < (1L << 31), "%s: too many images x planes", name);
-  (void)epr;
   *out = s;
   return DN_OK;
 }
@@ -330,12 +1005,78 @@ int gn_tensor(const char* name, const char* which, dn_tensor t, const GnShape& s
 long gn_part_bytes(const GnShape& s, int dtype) {
   return (long)s.N * s.P * s.nseg * (dtype == DN_BF16 ? 16 : 8) * (long)sizeof(float2);
 }
-long gn_workspace(const GnShape& s, int dtype) { return gn_part_bytes(s, dtype) + (long)s.N * s.G * (long)sizeof(float2) + 256; }
+// Whether the one-pass form takes this shape with R pieces per thread, and its plan.
+bool gn_fused_plan(const GnShape& s, int dtype, int r, GnFused* f) {
+  const int epr = dtype == DN_BF16 ? 16 : 8;
+  f->s = s;
+  const int seg = GNF_THREADS * r;
+  const int nseg = (s.npieces + seg - 1) / seg;
+  f->s.seg_len = ((s.npieces / 2 + nseg - 1) / nseg) * 2;
+  f->s.nseg = (s.npieces + f->s.seg_len - 1) / f->s.seg_len;
+  int a = s.cpg, b = epr;
+  while (b) { const int t = a % b; a = b; b = t; }
+  f->m = a;
+  f->ncell = epr / a;
+  f->ps = std::min(s.P, s.cpg / a);              // lcm(cpg, epr) / epr planes
+  f->nsets = (s.P + f->ps - 1) / f->ps;
+  const long k = (long)f->ps * f->s.nseg;
+  f->shards = (int)std::max(1L, std::min<long>(GNF_SHARDS, GNF_WAITING / std::max(1L, k - 1)));
+  f->d_most = gn_divisor(k);
+  f->d_shards = gn_divisor(f->shards);
+  f->d_nsets = gn_divisor(f->nsets);
+  f->d_nseg = gn_divisor(f->s.nseg);
+  f->d_cpg = gn_divisor(s.cpg);
+  f->d_m = gn_divisor(f->m);
+  f->inv_total = 1.0 / ((double)s.cpg * (s.npieces / 2));
+  f->polls = dn_tune().gn_polls ? dn_tune().gn_polls - 1 : GNF_POLLS;
+  return k <= GNF_MAX_K && k * f->ncell <= GNF_MAX_CELLS && f->nsets * k <= GNF_MAX_BLOCKS && s.C <= 1 << 15;
+}
+constexpr int GNF_R = 8, GNF_R_BWD = 4;          // 64 KB of a tensor, or 32 KB of each of two, in a block's registers
+// counters and published words first, at fixed places whatever the shape; the three-launch form's partials, and the partials of
+// the parameter gradients, behind them
+long gn_workspace(const GnShape& s, int dtype) {
+  GnFused f;
+  const bool both = gn_fused_plan(s, dtype, GNF_R, &f) && gn_fused_plan(s, dtype, GNF_R_BWD, &f);
+  const long chunks = both ? (long)s.P * gn_param_chunks(f.s) * (dtype == DN_BF16 ? 16 : 8) * (long)sizeof(double2) : 0;
+  const long parts = std::max(gn_part_bytes(s, dtype), both ? gn_part_bytes(f.s, dtype) + chunks : 0);
+  return GNF_END + parts + (long)s.N * s.G * (long)sizeof(float2) + 256;
+}
+void gn_fused_workspace(GnFused* f, void* workspace) {
+  char* w = (char*)workspace;
+  f->ctrl = (unsigned*)w;
+  f->depart = (unsigned*)(w + GNF_CTRL_BYTES);
+  f->list = (unsigned long long*)(w + GNF_LIST0);
+  f->slot = (unsigned long long*)(w + GNF_SLOT0);
+}
+// launch(grid) for as many images at a time as a launch takes; every shard gets the same number of blocks
+template <typename F> void gn_fused_each(GnFused* f, F launch) {
+  const long k = (long)f->ps * f->s.nseg;
+  const int most = (int)std::min<long>(f->s.N, GNF_MAX_BLOCKS / (f->nsets * k));
+  for (f->image0 = 0; f->image0 < f->s.N; f->image0 += most) {
+    f->images = std::min(most, f->s.N - f->image0);
+    const long clusters = (long)f->images * f->nsets;
+    launch(dim3((unsigned)((clusters + f->shards - 1) / f->shards * f->shards * k)));
+  }
+}
 
 template <typename T, int ACT>
 void gn_forward_launch(dn_tensor x, dn_tensor a, const GnShape& s, const float* gamma, const float* beta, float eps, float* mean,
-                       float* rstd, float* scale, float* shift, float2* part, hipStream_t st) {
+                       float* rstd, float* scale, float* shift, void* workspace, int dtype, hipStream_t st) {
   constexpr int EPR = RecTraits<T>::EPR;
+  GnFused f;
+  if (gn_fused_plan(s, dtype, GNF_R, &f)) {
+    gn_fused_workspace(&f, workspace);
+    const GnForward o{x.base, a.base, x.planes_total, x.plane0, a.planes_total, a.plane0, gamma, beta, eps, mean, rstd, scale, shift};
+    const int rows = (f.s.seg_len + GNF_THREADS - 1) / GNF_THREADS;            // pieces of a thread
+    gn_fused_each(&f, [&](dim3 grid) {
+      if (rows <= 2) hipLaunchKernelGGL((gn_fused_kernel<T, ACT, 2>), grid, dim3(GNF_THREADS), 0, st, f, o);
+      else if (rows <= 4) hipLaunchKernelGGL((gn_fused_kernel<T, ACT, 4>), grid, dim3(GNF_THREADS), 0, st, f, o);
+      else if (rows <= 6) hipLaunchKernelGGL((gn_fused_kernel<T, ACT, 6>), grid, dim3(GNF_THREADS), 0, st, f, o);
+      else hipLaunchKernelGGL((gn_fused_kernel<T, ACT, GNF_R>), grid, dim3(GNF_THREADS), 0, st, f, o);
+    });
+    return;
+  }
+  float2* part = (float2*)((char*)workspace + GNF_END);
   const dim3 grid((unsigned)((long)s.N * s.P * s.nseg));
   hipLaunchKernelGGL((gn_stats_kernel<T>), grid, dim3(GN_THREADS), 0, st, (const unsigned char*)x.base, x.planes_total, x.plane0, s, part);
   hipLaunchKernelGGL((gn_finalize_kernel<EPR>), dim3((unsigned)((long)s.N * s.G)), dim3(GN_THREADS), 0, st, part, s, gamma, beta, eps, mean,
@@ -345,8 +1086,28 @@ void gn_forward_launch(dn_tensor x, dn_tensor a, const GnShape& s, const float* 
 }
 template <typename T, int ACT>
 void gn_backward_launch(dn_tensor g, dn_tensor x, dn_tensor dx, const GnShape& s, const float* gamma, const float* mean, const float* rstd,
-                        const float* scale, const float* shift, float* dgamma, float* dbeta, float2* part, float2* coef, hipStream_t st) {
+                        const float* scale, const float* shift, float* dgamma, float* dbeta, void* workspace, int dtype,
+                        hipStream_t st) {
   constexpr int EPR = RecTraits<T>::EPR;
+  float2* part = (float2*)((char*)workspace + GNF_END);
+  GnFused f;
+  if (gn_fused_plan(s, dtype, GNF_R_BWD, &f)) {
+    gn_fused_workspace(&f, workspace);
+    const GnBackward o{g.base, x.base, dx.base, g.planes_total, g.plane0, x.planes_total, x.plane0, dx.planes_total, dx.plane0,
+                       gamma, mean, rstd, scale, shift, part};
+    const int rows = (f.s.seg_len + GNF_THREADS - 1) / GNF_THREADS;
+    gn_fused_each(&f, [&](dim3 grid) {
+      if (rows <= 1) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, 1>), grid, dim3(GNF_THREADS), 0, st, f, o);
+      else if (rows <= 2) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, 2>), grid, dim3(GNF_THREADS), 0, st, f, o);
+      else if (rows <= 3) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, 3>), grid, dim3(GNF_THREADS), 0, st, f, o);
+      else hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, GNF_R_BWD>), grid, dim3(GNF_THREADS), 0, st, f, o);
+    });
+    const int chunks = gn_param_chunks(f.s);
+    hipLaunchKernelGGL((gn_bwd_param_chunk_kernel<EPR>), dim3(s.P, chunks), dim3(GN_THREADS), 0, st, part, f.s, chunks, f.depart,
+                       (double2*)((char*)part + gn_part_bytes(f.s, dtype)), dgamma, dbeta);
+    return;
+  }
+  float2* coef = (float2*)((char*)workspace + GNF_END + gn_part_bytes(s, dtype));
   const dim3 grid((unsigned)((long)s.N * s.P * s.nseg));
   hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, ACT>), grid, dim3(GN_THREADS), 0, st, (const unsigned char*)g.base, g.planes_total, g.plane0,
                      (const unsigned char*)x.base, x.planes_total, x.plane0, s, mean, rstd, scale, shift, part);
@@ -388,11 +1149,11 @@ int dn_group_norm_act(dn_tensor x, dn_tensor a, int N, int H, int W, int groups,
   if (N == 0) return DN_OK;
   if ((rc = gn_tensor("dn_group_norm_act", "x", x, s)) || (rc = gn_tensor("dn_group_norm_act", "a", a, s))) return rc;
   DN_CHECK_ARG(gamma && beta && mean && rstd && scale && shift, "dn_group_norm_act: null vector");
-  DN_CHECK_ARG(eps > 0.f && eps < 1e30f, "dn_group_norm_act: eps must be positive");
+  DN_CHECK_ARG(eps >= 1e-30f && eps <= 1e30f, "dn_group_norm_act: eps must be within 1e-30 and 1e30");
   DN_CHECK_ARG(act >= DN_ACT_NONE && act <= DN_ACT_SILU, "dn_group_norm_act: bad activation %d", act);
   DN_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= gn_workspace(s, dtype),
                "dn_group_norm_act: workspace of %ld bytes, %ld needed (16-byte aligned)", workspace_bytes, gn_workspace(s, dtype));
-#define GN_CALL(T, A) (gn_forward_launch<T, A>(x, a, s, gamma, beta, eps, mean, rstd, scale, shift, (float2*)workspace, (hipStream_t)stream))
+#define GN_CALL(T, A) (gn_forward_launch<T, A>(x, a, s, gamma, beta, eps, mean, rstd, scale, shift, workspace, dtype, (hipStream_t)stream))
   GN_DISPATCH(dtype, act, GN_CALL)
 #undef GN_CALL
   DN_LAUNCH_CHECK();
@@ -413,9 +1174,7 @@ int dn_group_norm_act_backward(dn_tensor g, dn_tensor x, dn_tensor dx, int N, in
   DN_CHECK_ARG(act >= DN_ACT_NONE && act <= DN_ACT_SILU, "dn_group_norm_act_backward: bad activation %d", act);
   DN_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= gn_workspace(s, dtype),
                "dn_group_norm_act_backward: workspace of %ld bytes, %ld needed (16-byte aligned)", workspace_bytes, gn_workspace(s, dtype));
-  float2* part = (float2*)workspace;
-  float2* coef = (float2*)((char*)workspace + gn_part_bytes(s, dtype));
-#define GN_CALL(T, A) (gn_backward_launch<T, A>(g, x, dx, s, gamma, mean, rstd, scale, shift, dgamma, dbeta, part, coef, (hipStream_t)stream))
+#define GN_CALL(T, A) (gn_backward_launch<T, A>(g, x, dx, s, gamma, mean, rstd, scale, shift, dgamma, dbeta, workspace, dtype, (hipStream_t)stream))
   GN_DISPATCH(dtype, act, GN_CALL)
 #undef GN_CALL
   DN_LAUNCH_CHECK();

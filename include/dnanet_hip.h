@@ -257,7 +257,7 @@ int dn_bn_train_backward_apply_totals(dn_tensor g, dn_tensor y, const float* sca
  * torch.nn.functional.group_norm(x, groups, gamma, beta, eps) followed by the activation, per image and group over the
  * group's channels and H x W.  gamma / beta: [C]; mean / rstd: [N][groups]; scale / shift: [N][dn_channel_pad(C)], zero past
  * C: gamma * rstd and beta - mean * scale, kept for the backward pass.  C is a multiple of groups (groups need not fill
- * records), H * W <= 2^25, eps > 0.  a may be x.  N = 0 returns without a launch.
+ * records), H * W <= 2^25, 1e-30 <= eps <= 1e30.  a may be x.  N = 0 returns without a launch.
  * workspace: dn_group_norm_workspace_bytes (-1: refused sizes), 16-byte aligned; zero-filled by the caller before its first
  * use, left for the next call as each call needs it.  It may serve any sizes it is large enough for, one call at a time:
  * calls that overlap on the GPU need workspaces of their own. */

@@ -12,10 +12,11 @@ HALF = {"fp32": 0.0, "bf16": 2.0 ** -8}
 EPS = 1e-5
 
 # n, c, groups, h, w: one group per channel / one in all, groups inside records, across pieces, over whole planes, padded last
-# planes, one pixel, odd widths, planes of several segments
+# planes, one pixel, odd widths, planes of several segments, groups over several planes of several segments, a last set of planes
+# shorter than the others, more segments than one cluster of blocks takes
 SHAPES = [(1, 8, 1, 1, 1), (2, 8, 8, 1, 1), (1, 8, 2, 1, 3), (3, 24, 8, 5, 37), (2, 40, 5, 3, 64), (2, 48, 16, 6, 33), (1, 32, 8, 5, 1024),
           (2, 32, 32, 2, 129), (1, 64, 1, 5, 520), (2, 72, 9, 1, 250), (1, 512, 8, 5, 16), (17, 16, 4, 6, 96), (1, 20, 4, 2, 4099),
-          (3, 96, 3, 5, 700)]
+          (3, 96, 3, 5, 700), (1, 60, 5, 4, 1500), (2, 60, 5, 1, 40), (1, 16, 2, 7, 20001), (2, 1024, 1, 5, 32), (3, 512, 2, 6, 256)]
 ACTS = {"none": lambda z: z, "relu": torch.relu, "silu": F.silu}
 
 
@@ -340,3 +341,54 @@ def test_refusals(gpu_device):
     with pytest.raises(ValueError, match="stats.mean"):
         stats.groups = 4
         group_norm_act_backward(a.ref(32), x.ref(32), one, stats)
+
+
+GIVE_UP = """
+import hashlib, sys, torch
+sys.path[:0] = [{root!r}, {tests!r}]
+from test_group_norm_gpu import digests
+print("DIGESTS", digests())
+"""
+EXCHANGE_SHAPES = [(2, 40, 5, 3, 2000), (3, 64, 2, 5, 1500), (2, 60, 5, 4, 1500), (16, 32, 8, 6, 4096), (30, 128, 8, 5, 1024), (130, 512, 8, 6, 256)]
+
+
+def digests():
+    """Hashes of forward and (in place) backward results at shapes whose groups are spread over several blocks."""
+    import hashlib
+    from dnanet_amd import hip
+    from dnanet_amd.group_norm import group_norm_act, group_norm_act_backward
+    from dnanet_amd.hip import PlaneBuffer
+    out = []
+    for dtype in (hip.BF16, hip.F32):
+        for n, c, groups, h, w in EXCHANGE_SHAPES:
+            gen = torch.Generator(device="cuda").manual_seed(n + c)
+            x, g = (PlaneBuffer(n, hip.planes(c, dtype), h, w, dtype, "cuda") for _ in range(2))
+            for b in (x, g):
+                b.data.copy_(torch.randn(b.data.shape, generator=gen, device="cuda"))
+                if c % hip.epr(dtype):
+                    b.data[:, -1, :, :, c % hip.epr(dtype):] = 0
+            gamma, beta = torch.rand(c, generator=gen, device="cuda") + 0.5, torch.rand(c, generator=gen, device="cuda")
+            for act in ("relu", "silu"):
+                a, stats = group_norm_act(x.ref(c), gamma, beta, groups, EPS, act)
+                mine = PlaneBuffer.wrap(g.data.clone())
+                _, dgamma, dbeta = group_norm_act_backward(mine.ref(c), x.ref(c), gamma, stats, out=mine.ref(c))
+                md5 = hashlib.md5()
+                for t in (a.data, mine.data, dgamma, dbeta, stats.mean, stats.rstd, stats.scale, stats.shift):
+                    md5.update(t.contiguous().view(torch.uint8).cpu().numpy().tobytes())
+                out.append(md5.hexdigest()[:12])
+    return out
+
+
+def test_blocks_that_give_up_waiting(gpu_device):
+    """A block that does not find the sums it waits for leaves its segment to the launch's last block: with no patience at all
+    (one look) the results are the same bits."""
+    import os
+    import subprocess
+    import sys
+    tests = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, DN_TUNE_GN_POLLS="1")
+    run = subprocess.run([sys.executable, "-c", GIVE_UP.format(root=os.path.dirname(tests), tests=tests)], env=env, capture_output=True,
+                         text=True, timeout=100)
+    assert run.returncode == 0, run.stderr[-2000:]
+    impatient = run.stdout.split("DIGESTS ", 1)[1].strip()
+    assert impatient == str(digests())
