@@ -27,12 +27,13 @@ def parse_activation(activation: str) -> int:
 
 class GroupNormStats:
     """What a forward pass leaves for its backward pass: ``mean`` / ``rstd`` (N, groups), the fused ``scale`` / ``shift``
-    (N, channels padded to 32), and how they were made."""
+    (N, channels padded to 32), and how they were made.  The four lie one after the other in ``flat`` where a forward call
+    made them, and become tensors of their own when they are asked for."""
 
-    __slots__ = ("mean", "rstd", "scale", "shift", "groups", "activation")
+    __slots__ = ("flat", "_parts", "_shape", "groups", "activation")
 
     def __init__(self, mean: torch.Tensor, rstd: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor, groups: int, activation: str):
-        self.mean, self.rstd, self.scale, self.shift = mean, rstd, scale, shift
+        self.flat, self._parts, self._shape = None, (mean, rstd, scale, shift), None
         self.groups, self.activation = groups, activation
 
     @staticmethod
@@ -41,31 +42,58 @@ class GroupNormStats:
 
     @classmethod
     def from_flat(cls, flat: torch.Tensor, n: int, channels: int, groups: int, activation: str) -> "GroupNormStats":
-        """Views into ``floats(n, channels, groups)`` consecutive fp32 values."""
+        """Over ``floats(n, channels, groups)`` consecutive fp32 values."""
+        self = cls.__new__(cls)
+        self.flat, self._parts, self._shape = flat, None, (n, groups, hip.channel_pad(channels))
+        self.groups, self.activation = groups, activation
+        return self
+
+    def _part(self, k: int) -> torch.Tensor:
+        if self._parts is not None:
+            return self._parts[k]
+        n, groups, pad = self._shape
+        if k < 2:
+            return self.flat.as_strided((n, groups), (groups, 1), self.flat.storage_offset() + k * n * groups)
+        return self.flat.as_strided((n, pad), (pad, 1), self.flat.storage_offset() + n * (2 * groups + (k - 2) * pad))
+
+    mean = property(lambda self: self._part(0))
+    rstd = property(lambda self: self._part(1))
+    scale = property(lambda self: self._part(2))
+    shift = property(lambda self: self._part(3))
+
+    def _pointers(self, n: int, channels: int, groups: int, device: torch.device) -> Tuple[int, int, int, int]:
+        """Device pointers of the four, checked against a call's sizes."""
         pad = hip.channel_pad(channels)
-        a, b = n * groups, n * pad
-        mean, rstd, scale, shift = flat.split_with_sizes((a, a, b, b))
-        return cls(mean.view(n, groups), rstd.view(n, groups), scale.view(n, pad), shift.view(n, pad), groups, activation)
+        if self._parts is None:
+            if self._shape != (n, groups, pad):
+                raise ValueError(f"stats.mean is of {self._shape[0]} images and {self._shape[1]} groups, the call of {n} and {groups}")
+            base = _vector(self.flat, (2 * n * (groups + pad),), device, "stats.flat")
+            return base, base + 4 * n * groups, base + 8 * n * groups, base + 8 * n * groups + 4 * n * pad
+        mean, rstd, scale, shift = self._parts
+        return (_vector(mean, (n, groups), device, "stats.mean"), _vector(rstd, (n, groups), device, "stats.rstd"),
+                _vector(scale, (n, pad), device, "stats.scale"), _vector(shift, (n, pad), device, "stats.shift"))
 
 
 _workspaces: Dict[Tuple[int, int], torch.Tensor] = {}
 
 
-def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
+def _workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
     """Zero-filled before its first use, as the library asks.  Calls on one stream follow each other and share a workspace.  A
     call under HIP-graph capture gets one of its own inside the graph (zeroed there on every replay): two graphs captured on
     the same stream may be replayed at the same time."""
     if torch.cuda.is_current_stream_capturing():
         return torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
-    ws = _workspaces.get(key)
+    ws = _workspaces.get((device.index, stream))
     if ws is None or ws.numel() < nbytes:
-        ws = _workspaces[key] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+        ws = _workspaces[device.index, stream] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
     return ws
 
 
+_HERE = nullcontext()
+
+
 def _on(device: torch.device):
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _owner(ref: DnTensor, what: str) -> PlaneBuffer:
@@ -114,13 +142,12 @@ def group_norm_act(x: DnTensor, gamma: torch.Tensor, beta: torch.Tensor, groups:
     if stats is None:
         flat = torch.empty(GroupNormStats.floats(src.n, c, groups), dtype=torch.float32, device=dev)
         stats = GroupNormStats.from_flat(flat, src.n, c, groups, activation)
-    pad = hip.channel_pad(c)
-    vectors = [_vector(stats.mean, (src.n, groups), dev, "stats.mean"), _vector(stats.rstd, (src.n, groups), dev, "stats.rstd"),
-               _vector(stats.scale, (src.n, pad), dev, "stats.scale"), _vector(stats.shift, (src.n, pad), dev, "stats.shift")]
+    vectors = stats._pointers(src.n, c, groups, dev)
     with _on(dev):
-        ws = _workspace(dev, need) if workspace is None else workspace
+        stream = hip.raw_stream(dev)
+        ws = _workspace(dev, stream, need) if workspace is None else workspace
         hip.check(hip.lib.dn_group_norm_act(x, out, src.n, src.h, src.w, groups, g, b, eps, act, *vectors, ws.data_ptr(), ws.numel(),
-                                            src.dtype, hip.stream_ptr()))
+                                            src.dtype, stream))
     stats.groups, stats.activation = groups, activation
     return dst, stats
 
@@ -147,12 +174,11 @@ def group_norm_act_backward(g: DnTensor, x: DnTensor, gamma: torch.Tensor, stats
         dgamma = torch.empty(c, dtype=torch.float32, device=dev)
     if dbeta is None:
         dbeta = torch.empty(c, dtype=torch.float32, device=dev)
-    pad = hip.channel_pad(c)
-    vectors = [_vector(stats.mean, (src.n, groups), dev, "stats.mean"), _vector(stats.rstd, (src.n, groups), dev, "stats.rstd"),
-               _vector(stats.scale, (src.n, pad), dev, "stats.scale"), _vector(stats.shift, (src.n, pad), dev, "stats.shift")]
+    vectors = stats._pointers(src.n, c, groups, dev)
     dg, db = _vector(dgamma, (c,), dev, "dgamma"), _vector(dbeta, (c,), dev, "dbeta")
     with _on(dev):
-        ws = _workspace(dev, need) if workspace is None else workspace
+        stream = hip.raw_stream(dev)
+        ws = _workspace(dev, stream, need) if workspace is None else workspace
         hip.check(hip.lib.dn_group_norm_act_backward(g, x, out, src.n, src.h, src.w, groups, ga, *vectors, parse_activation(stats.activation),
-                                                     dg, db, ws.data_ptr(), ws.numel(), src.dtype, hip.stream_ptr()))
+                                                     dg, db, ws.data_ptr(), ws.numel(), src.dtype, stream))
     return dst, dgamma, dbeta

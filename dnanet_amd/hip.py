@@ -157,6 +157,11 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def raw_stream(device: torch.device) -> int:
+    """``stream_ptr`` of a device, without a Stream object (which costs more than a launch)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     if t is None:
         return None

@@ -22,6 +22,10 @@ _DTYPE = {torch.float32: F32, torch.bfloat16: BF16}
 _BLOCK = 256                     # elements of an 8-bit state block; a tensor's moments start at a multiple of it
 
 
+_data_ptr = torch.Tensor.data_ptr
+_HERE = nullcontext()
+
+
 def _blocks(n: int) -> int:
     return (n + _BLOCK - 1) // _BLOCK
 
@@ -78,6 +82,7 @@ class HipAdamW:
                 raise ValueError(f"{len(given)} gradients for {len(group['params'])} parameters")
             self._given += given
             self.param_groups.append(group)
+        self._all_given = all(g is not None for g in self._given)
         self._params: List[torch.Tensor] = [p for g in self.param_groups for p in g["params"]]
         if not self._params:
             raise ValueError("no parameters")
@@ -127,10 +132,11 @@ class HipAdamW:
         decays = [g["weight_decay"] for g in self.param_groups]
         if self._table is not None and self.model is not None and decays == self._decays:
             return                               # a model's arenas stay where they are
-        grads = [p.grad if g is None else g for p, g in zip(self._params, self._given)]
-        pointers = [t.data_ptr() for t in grads if t is not None] + [p.data_ptr() for p in self._params]
-        if self._table is not None and decays == self._decays and pointers == self._pointers and \
-                all(map(is_, grads, [r and r() for r in self._grads])):
+        grads = self._given if self._all_given else [p.grad if g is None else g for p, g in zip(self._params, self._given)]
+        pointers = list(map(_data_ptr, self._params))
+        pointers += map(_data_ptr, grads if self._all_given else [g for g in grads if g is not None])
+        if self._table is not None and pointers == self._pointers and decays == self._decays and \
+                (self._all_given or all(map(is_, grads, [r and r() for r in self._grads]))):
             return
         self._check_params()
         for p, g in zip(self._params, grads):
@@ -180,9 +186,9 @@ class HipAdamW:
         state = (self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(), hip.ptr(self.exp_avg_scale), hip.ptr(self.exp_avg_sq_scale),
                  self.state_bits)
         zero = 1 if self.model is not None else 0
-        guard = nullcontext() if self.device.index == torch.cuda.current_device() else torch.cuda.device(self.device)
+        guard = _HERE if self.device.index == torch.cuda.current_device() else torch.cuda.device(self.device)
         with guard:
-            stream = hip.stream_ptr()
+            stream = hip.raw_stream(self.device)
             clip = None
             if self._clip is not None:
                 clip = self._clip.data_ptr()
