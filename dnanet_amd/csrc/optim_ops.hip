@@ -52,14 +52,13 @@ struct AdamwArgs {
   const long long* step_dev;                  // with hyper
 };
 
-// index of the tensor that owns block b: blocks of a tensor are consecutive, block0 ascends
+// index of the tensor that owns block b (blocks of a tensor are consecutive, block0 ascends): every lane compares two entries,
+// one load's latency instead of seven for a binary search
 __device__ __forceinline__ int adamw_find(const AdamwList& l, unsigned b) {
-  int lo = 0, hi = l.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (l.e[mid].block0 <= b) lo = mid; else hi = mid - 1;
-  }
-  return lo;
+  const int lane = threadIdx.x & 63;
+  const bool first = lane < l.count && l.e[min(lane, ADAMW_MAX - 1)].block0 <= b;
+  const bool second = lane + 64 < l.count && l.e[min(lane + 64, ADAMW_MAX - 1)].block0 <= b;
+  return __popcll(__ballot(first)) + __popcll(__ballot(second)) - 1;
 }
 
 __device__ __forceinline__ unsigned adamw_hash(unsigned x) {
@@ -118,32 +117,84 @@ __device__ __forceinline__ AdamwScalars adamw_scalars(const AdamwArgs& a) {
   return s;
 }
 
+// p (1 - lr decay) - step m / (sqrt(v) / sqrt(1 - beta2^t) + eps); square root and reciprocal to 1 ulp
+__device__ __forceinline__ float adamw_update(float p, float m, float v, float keep, const AdamwScalars& s, float eps) {
+  const float denom = fmaf(__builtin_amdgcn_sqrtf(v), s.inv_sqrt_bc2, eps);
+  return fmaf(-s.step_size * m, __builtin_amdgcn_rcpf(denom), p * keep);
+}
+
+// A row is 256 elements, four of each lane of a wave; a block's waves take the rows of its chunk in turn.
+constexpr int ADAMW_ROW = 256, ADAMW_WAVES = ADAMW_THREADS / 64;
+
+struct AdamwRow32 { float p[4], g[4], m[4], v[4]; };
+__device__ __forceinline__ void adamw_row32(AdamwRow32& r, const AdamwArgs& a, const AdamwScalars& s, float keep) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float g = r.g[j] * s.coef;
+    r.m[j] = fmaf(a.beta1, r.m[j], a.omb1 * g);
+    r.v[j] = fmaf(a.beta2, r.v[j], a.omb2 * g * g);
+    r.p[j] = adamw_update(r.p[j], r.m[j], r.v[j], keep, s, a.eps);
+  }
+}
+// `rows` whole rows of an aligned tensor from element i of lane 0 on, N at a time in flight
+template <typename P, typename G, int N>
+__device__ __forceinline__ void adamw_rows32(const AdamwEntry& e, long first, int rows, float* m, float* v, const AdamwArgs& a,
+                                             const AdamwScalars& s, float keep) {
+  for (int row = threadIdx.x >> 6; row < rows; row += ADAMW_WAVES * N) {
+    AdamwRow32 r[N];
+    const long i = first + (long)row * ADAMW_ROW + (threadIdx.x & 63) * 4;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (row + k * ADAMW_WAVES < rows) {
+        const long at = i + (long)k * ADAMW_WAVES * ADAMW_ROW;
+        adamw_load<P>(e.p, at, 4, true, r[k].p);
+        adamw_load<G>(e.g, at, 4, true, r[k].g);
+        adamw_load<float>(m, at, 4, true, r[k].m);
+        adamw_load<float>(v, at, 4, true, r[k].v);
+      }
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (row + k * ADAMW_WAVES < rows) {
+        const long at = i + (long)k * ADAMW_WAVES * ADAMW_ROW;
+        adamw_row32(r[k], a, s, keep);
+        adamw_store<P>(e.p, at, 4, true, r[k].p);
+        adamw_store<float>(m, at, 4, true, r[k].m);
+        adamw_store<float>(v, at, 4, true, r[k].v);
+        if (a.zero_grad) {
+          const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+          adamw_store<G>(e.g, at, 4, true, zero);
+        }
+      }
+  }
+}
+
 __global__ __launch_bounds__(ADAMW_THREADS) void adamw_kernel(AdamwList list, float* exp_avg, float* exp_avg_sq, AdamwArgs a) {
-  const int t = adamw_find(list, blockIdx.x);
-  const AdamwEntry e = list.e[t];
+  const AdamwEntry e = list.e[adamw_find(list, blockIdx.x)];
   const AdamwScalars s = adamw_scalars(a);
-  const bool pb = e.flags & ADAMW_P_BF16, gb = e.flags & ADAMW_G_BF16, vec = e.flags & ADAMW_VECTOR;
   const float keep = 1.f - s.lr * e.decay;
   float* m = exp_avg + (long)e.state * 256;
   float* v = exp_avg_sq + (long)e.state * 256;
   const long lo = (long)(blockIdx.x - e.block0) * ADAMW_CHUNK, hi = min(e.n, lo + ADAMW_CHUNK);
-  for (long i = lo + threadIdx.x * 4; i < hi; i += ADAMW_THREADS * 4) {
+  const bool pb = e.flags & ADAMW_P_BF16, gb = e.flags & ADAMW_G_BF16, vec = e.flags & ADAMW_VECTOR;
+  const int rows = vec ? (int)((hi - lo) / ADAMW_ROW) : 0;
+  if (pb) {
+    if (gb) adamw_rows32<__bf16, __bf16, 2>(e, lo, rows, m, v, a, s, keep);
+    else adamw_rows32<__bf16, float, 2>(e, lo, rows, m, v, a, s, keep);
+  } else {
+    if (gb) adamw_rows32<float, __bf16, 2>(e, lo, rows, m, v, a, s, keep);
+    else adamw_rows32<float, float, 2>(e, lo, rows, m, v, a, s, keep);
+  }
+  for (long i = lo + rows * ADAMW_ROW + threadIdx.x * 4; i < hi; i += ADAMW_THREADS * 4) {       // the rest, or an unaligned tensor
     const int count = (int)min(4L, hi - i);
-    float fp[4], fg[4], fm[4], fv[4];
-    adamw_load_any(e.p, pb, i, count, vec, fp);
-    adamw_load_any(e.g, gb, i, count, vec, fg);
-    adamw_load<float>(m, i, count, true, fm);
-    adamw_load<float>(v, i, count, true, fv);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float g = fg[j] * s.coef;
-      fm[j] = fmaf(a.beta1, fm[j], a.omb1 * g);
-      fv[j] = fmaf(a.beta2, fv[j], a.omb2 * g * g);
-      fp[j] = fp[j] * keep - s.step_size * fm[j] / (sqrtf(fv[j]) * s.inv_sqrt_bc2 + a.eps);
-    }
-    adamw_store_any(e.p, pb, i, count, vec, fp);
-    adamw_store<float>(m, i, count, true, fm);
-    adamw_store<float>(v, i, count, true, fv);
+    AdamwRow32 r;
+    adamw_load_any(e.p, pb, i, count, vec, r.p);
+    adamw_load_any(e.g, gb, i, count, vec, r.g);
+    adamw_load<float>(m, i, count, true, r.m);
+    adamw_load<float>(v, i, count, true, r.v);
+    adamw_row32(r, a, s, keep);
+    adamw_store_any(e.p, pb, i, count, vec, r.p);
+    adamw_store<float>(m, i, count, true, r.m);
+    adamw_store<float>(v, i, count, true, r.v);
     if (a.zero_grad) {
       const float zero[4] = {0.f, 0.f, 0.f, 0.f};
       adamw_store_any(e.g, gb, i, count, vec, zero);
@@ -164,72 +215,140 @@ __device__ __forceinline__ int adamw_exponent(float amax) {
   return max((int)((__float_as_uint(amax) + 0x1FFFFFu) >> 23) - 127 - 8, -126);
 }
 
+// Largest of a non-negative value over the wave, in every lane: DPP moves within and across the rows of 16, no LDS
+__device__ __forceinline__ float adamw_wave_max(float v) {
+#define ADAMW_DPP(ctrl) v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, false)))
+  ADAMW_DPP(0xB1);       // quad_perm [1,0,3,2]
+  ADAMW_DPP(0x4E);       // quad_perm [2,3,0,1]
+  ADAMW_DPP(0x124);      // row_ror:4
+  ADAMW_DPP(0x128);      // row_ror:8
+  ADAMW_DPP(0x142);      // row_bcast:15 -> the next row (rows 1, 3 hold two rows' maximum)
+  ADAMW_DPP(0x143);      // row_bcast:31 -> rows 2, 3 (row 3 holds all)
+#undef ADAMW_DPP
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
+// One row of a tensor with 8-bit moments: codes and scales in, codes and scales out.  count: elements of this lane that exist.
+struct AdamwRow8 {
+  float p[4], g[4];
+  unsigned cm, cv;
+  float ms, vs;
+};
+__device__ __forceinline__ void adamw_row8(AdamwRow8& r, int count, unsigned place, const AdamwArgs& a, const AdamwScalars& s, float keep) {
+  const double ms = (double)r.ms * a.dbeta1, vs = (double)r.vs * a.dbeta2, coef = (double)s.coef;
+  const float om[4] = {__builtin_amdgcn_cvt_f32_fp8(r.cm, 0), __builtin_amdgcn_cvt_f32_fp8(r.cm, 1), __builtin_amdgcn_cvt_f32_fp8(r.cm, 2),
+                       __builtin_amdgcn_cvt_f32_fp8(r.cm, 3)};
+  const float ov[4] = {__builtin_amdgcn_cvt_f32_fp8(r.cv, 0), __builtin_amdgcn_cvt_f32_fp8(r.cv, 1), __builtin_amdgcn_cvt_f32_fp8(r.cv, 2),
+                       __builtin_amdgcn_cvt_f32_fp8(r.cv, 3)};
+  float fm[4], fv[4], am = 0.f, av = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const double g = (double)r.g[j] * coef;
+    fm[j] = j < count ? (float)fma((double)om[j], ms, a.domb1 * g) : 0.f;
+    fv[j] = j < count ? (float)fma((double)ov[j], vs, a.domb2 * g * g) : 0.f;
+    const float mag = fabsf(fm[j]);
+    am = fmaxf(am, mag <= 3.4028235e38f ? mag : 0.f);
+    av = fmaxf(av, fv[j] <= 3.4028235e38f ? fv[j] : 0.f);
+  }
+  am = adamw_wave_max(am);
+  av = adamw_wave_max(av);
+  const int em = adamw_exponent(am), ev = adamw_exponent(av);
+  const float im = __uint_as_float((unsigned)(127 - em) << 23), iv = __uint_as_float((unsigned)(127 - ev) << 23);      // 2^-k
+  r.cm = r.cv = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const unsigned h = adamw_hash(place + j);
+    unsigned c = adamw_encode(fabsf(fm[j]) * im, h & 0xFFFFu);
+    if (!(fabsf(fm[j]) <= 3.4028235e38f)) c = 0x7F;
+    if (fm[j] < 0.f) c |= 0x80u;
+    r.cm |= c << (8 * j);
+    c = adamw_encode(fv[j] * iv, h >> 16);
+    if (fv[j] > 0.f) c = max(c, 1u);
+    if (!(fv[j] <= 3.4028235e38f)) c = 0x7F;
+    r.cv |= c << (8 * j);
+    r.p[j] = adamw_update(r.p[j], fm[j], fv[j], keep, s, a.eps);
+  }
+  r.ms = am > 0.f ? __uint_as_float((unsigned)(127 + em) << 23) : 0.f;
+  r.vs = av > 0.f ? __uint_as_float((unsigned)(127 + ev) << 23) : 0.f;
+}
+
+struct Adamw8State {
+  unsigned char *m, *v;
+  float *ms, *vs;
+};
+template <typename P, typename G, int N>
+__device__ __forceinline__ void adamw_rows8(const AdamwEntry& e, long first, int rows, const Adamw8State& o, unsigned key, const AdamwArgs& a,
+                                            const AdamwScalars& s, float keep) {
+  const int lane = threadIdx.x & 63;
+  for (int row = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < rows; row += ADAMW_WAVES * N) {
+    AdamwRow8 r[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (row + k * ADAMW_WAVES < rows) {
+        const long base = first + (long)(row + k * ADAMW_WAVES) * ADAMW_ROW, at = base + lane * 4;
+        adamw_load<P>(e.p, at, 4, true, r[k].p);
+        adamw_load<G>(e.g, at, 4, true, r[k].g);
+        r[k].cm = *(const unsigned*)(o.m + at);
+        r[k].cv = *(const unsigned*)(o.v + at);
+        r[k].ms = o.ms[base >> 8];
+        r[k].vs = o.vs[base >> 8];
+      }
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (row + k * ADAMW_WAVES < rows) {
+        const long base = first + (long)(row + k * ADAMW_WAVES) * ADAMW_ROW, at = base + lane * 4;
+        adamw_row8(r[k], 4, (unsigned)at + key, a, s, keep);
+        adamw_store<P>(e.p, at, 4, true, r[k].p);
+        *(unsigned*)(o.m + at) = r[k].cm;
+        *(unsigned*)(o.v + at) = r[k].cv;
+        if (lane == 0) { o.ms[base >> 8] = r[k].ms; o.vs[base >> 8] = r[k].vs; }
+        if (a.zero_grad) {
+          const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+          adamw_store<G>(e.g, at, 4, true, zero);
+        }
+      }
+  }
+}
+
 __global__ __launch_bounds__(ADAMW_THREADS) void adamw8_kernel(AdamwList list, unsigned char* exp_avg, unsigned char* exp_avg_sq,
                                                                float* m_scale, float* v_scale, AdamwArgs a) {
-  const int t = adamw_find(list, blockIdx.x);
-  const AdamwEntry e = list.e[t];
+  const AdamwEntry e = list.e[adamw_find(list, blockIdx.x)];
   const AdamwScalars s = adamw_scalars(a);
-  const bool pb = e.flags & ADAMW_P_BF16, gb = e.flags & ADAMW_G_BF16, vec = e.flags & ADAMW_VECTOR;
   const float keep = 1.f - s.lr * e.decay;
   const unsigned key = e.state * 256u + s.step * 0x9E3779B9u + a.seed * 0x85EBCA6Bu;
+  const Adamw8State o{exp_avg + (long)e.state * 256, exp_avg_sq + (long)e.state * 256, m_scale + e.state, v_scale + e.state};
   const long lo = (long)(blockIdx.x - e.block0) * ADAMW_CHUNK, hi = min(e.n, lo + ADAMW_CHUNK);
+  const bool pb = e.flags & ADAMW_P_BF16, gb = e.flags & ADAMW_G_BF16, vec = e.flags & ADAMW_VECTOR;
+  const int rows = vec ? (int)((hi - lo) / ADAMW_ROW) : 0;
+  if (pb) {
+    if (gb) adamw_rows8<__bf16, __bf16, 2>(e, lo, rows, o, key, a, s, keep);
+    else adamw_rows8<__bf16, float, 2>(e, lo, rows, o, key, a, s, keep);
+  } else {
+    if (gb) adamw_rows8<float, __bf16, 2>(e, lo, rows, o, key, a, s, keep);
+    else adamw_rows8<float, float, 2>(e, lo, rows, o, key, a, s, keep);
+  }
   const int lane = threadIdx.x & 63;
-  // a wave owns a state block of 256 elements at a time, four per lane
-  for (long row = lo + (threadIdx.x >> 6) * 256; row < hi; row += ADAMW_THREADS * 4) {
-    const long i = row + lane * 4;
-    const int count = (int)max(0L, min(4L, hi - i));
-    const long at = (long)e.state * 256 + i;           // the state buffers hold whole blocks
-    const long block = (long)e.state + (row >> 8);
-    float fp[4], fg[4];
-    adamw_load_any(e.p, pb, i, count, vec, fp);
-    adamw_load_any(e.g, gb, i, count, vec, fg);
-    const unsigned cm = *(const unsigned*)(exp_avg + at), cv = *(const unsigned*)(exp_avg_sq + at);
-    const double ms = (double)m_scale[block] * a.dbeta1, vs = (double)v_scale[block] * a.dbeta2;
-    const float om[4] = {__builtin_amdgcn_cvt_f32_fp8(cm, 0), __builtin_amdgcn_cvt_f32_fp8(cm, 1), __builtin_amdgcn_cvt_f32_fp8(cm, 2),
-                         __builtin_amdgcn_cvt_f32_fp8(cm, 3)};
-    const float ov[4] = {__builtin_amdgcn_cvt_f32_fp8(cv, 0), __builtin_amdgcn_cvt_f32_fp8(cv, 1), __builtin_amdgcn_cvt_f32_fp8(cv, 2),
-                         __builtin_amdgcn_cvt_f32_fp8(cv, 3)};
-    float fm[4], fv[4], am = 0.f, av = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const double g = (double)fg[j] * (double)s.coef;
-      fm[j] = j < count ? (float)fma((double)om[j], ms, a.domb1 * g) : 0.f;
-      fv[j] = j < count ? (float)fma((double)ov[j], vs, a.domb2 * g * g) : 0.f;
-      const float mag = fabsf(fm[j]);
-      if (mag <= 3.4028235e38f) am = fmaxf(am, mag);
-      if (fv[j] <= 3.4028235e38f) av = fmaxf(av, fv[j]);
-    }
-#pragma unroll
-    for (int x = 32; x >= 1; x >>= 1) { am = fmaxf(am, __shfl_xor(am, x)); av = fmaxf(av, __shfl_xor(av, x)); }
-    const int em = adamw_exponent(am), ev = adamw_exponent(av);
-    const float im = __uint_as_float((unsigned)(127 - em) << 23), iv = __uint_as_float((unsigned)(127 - ev) << 23);      // 2^-k
-    unsigned om8 = 0, ov8 = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned h = adamw_hash((unsigned)(i + j) + key);
-      unsigned c = adamw_encode(fabsf(fm[j]) * im, h & 0xFFFFu);
-      if (!(fabsf(fm[j]) <= 3.4028235e38f)) c = 0x7F;
-      if (fm[j] < 0.f) c |= 0x80u;
-      om8 |= c << (8 * j);
-      c = adamw_encode(fv[j] * iv, h >> 16);
-      if (fv[j] > 0.f) c = max(c, 1u);
-      if (!(fv[j] <= 3.4028235e38f)) c = 0x7F;
-      ov8 |= c << (8 * j);
-      fp[j] = fp[j] * keep - s.step_size * fm[j] / (sqrtf(fv[j]) * s.inv_sqrt_bc2 + a.eps);
-    }
+  for (long base = lo + (rows + (threadIdx.x >> 6)) * ADAMW_ROW; base < hi; base += ADAMW_WAVES * ADAMW_ROW) {      // the rest, or an unaligned tensor
+    const long at = base + lane * 4;
+    const int count = (int)max(0L, min(4L, hi - at));
+    AdamwRow8 r;
+    adamw_load_any(e.p, pb, at, count, vec, r.p);
+    adamw_load_any(e.g, gb, at, count, vec, r.g);
+    r.cm = *(const unsigned*)(o.m + at);               // the state buffers hold whole blocks
+    r.cv = *(const unsigned*)(o.v + at);
+    r.ms = o.ms[base >> 8];
+    r.vs = o.vs[base >> 8];
+    adamw_row8(r, count, (unsigned)at + key, a, s, keep);
     if (count > 0) {
-      adamw_store_any(e.p, pb, i, count, vec, fp);
+      adamw_store_any(e.p, pb, at, count, vec, r.p);
+      *(unsigned*)(o.m + at) = r.cm;                   // places past the tensor's end are zero and stay zero
+      *(unsigned*)(o.v + at) = r.cv;
       if (a.zero_grad) {
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-        adamw_store_any(e.g, gb, i, count, vec, zero);
+        adamw_store_any(e.g, gb, at, count, vec, zero);
       }
-      *(unsigned*)(exp_avg + at) = om8;                // elements past the tensor's end are zero and stay zero
-      *(unsigned*)(exp_avg_sq + at) = ov8;
     }
-    if (lane == 0) {
-      m_scale[block] = am > 0.f ? ldexpf(1.f, em) : 0.f;
-      v_scale[block] = av > 0.f ? ldexpf(1.f, ev) : 0.f;
-    }
+    if (lane == 0) { o.ms[base >> 8] = r.ms; o.vs[base >> 8] = r.vs; }
   }
 }
 
@@ -257,8 +376,7 @@ __device__ __forceinline__ double adamw_block_sum(double v) {
   return v;
 }
 __global__ __launch_bounds__(ADAMW_THREADS) void grad_norm_kernel(AdamwList list, double* partial) {
-  const int t = adamw_find(list, blockIdx.x);
-  const AdamwEntry e = list.e[t];
+  const AdamwEntry e = list.e[adamw_find(list, blockIdx.x)];
   const bool gb = e.flags & ADAMW_G_BF16, vec = e.flags & ADAMW_VECTOR;
   const long lo = (long)(blockIdx.x - e.block0) * ADAMW_CHUNK, hi = min(e.n, lo + ADAMW_CHUNK);
   double sum = 0.0;
