@@ -117,9 +117,12 @@ __device__ __forceinline__ AdamwScalars adamw_scalars(const AdamwArgs& a) {
   return s;
 }
 
-// p (1 - lr decay) - step m / (sqrt(v) / sqrt(1 - beta2^t) + eps); square root and reciprocal to 1 ulp
+// p (1 - lr decay) - step m / (sqrt(v) / sqrt(1 - beta2^t) + eps); square root and reciprocal to 1 ulp.  The square root
+// instruction takes a denormal v for zero, which matters where eps is zero: v below 2^-96 is brought up by 2^64.
 __device__ __forceinline__ float adamw_update(float p, float m, float v, float keep, const AdamwScalars& s, float eps) {
-  const float denom = fmaf(__builtin_amdgcn_sqrtf(v), s.inv_sqrt_bc2, eps);
+  const bool tiny = v < 0x1p-96f;
+  const float root = __builtin_amdgcn_sqrtf(tiny ? v * 0x1p64f : v);
+  const float denom = fmaf(tiny ? root * 0x1p-32f : root, s.inv_sqrt_bc2, eps);
   return fmaf(-s.step_size * m, __builtin_amdgcn_rcpf(denom), p * keep);
 }
 
@@ -202,22 +205,24 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_kernel(AdamwList list, fl
   }
 }
 
-// magnitude over the block's scale -> e4m3 code, rounded up where the 16 random bits say so
-__device__ __forceinline__ unsigned adamw_encode(float y, unsigned bits) {
-  const bool small = y < 0.015625f;                    // below the smallest normal value (2^-6) the code steps are even: 2^-6 + y has
-  const float z = small ? y + 0.015625f : y;           // the same steps as a normal number
-  const int code = (int)((__float_as_uint(z) + (bits << 4)) >> 20) - (small ? 121 * 8 : 120 * 8);
-  return (unsigned)min(code, 126);
+// Two values over their block's scale -> e4m3 codes in bytes 2 * HALF and up of `codes`.  The conversion adds 20 bits of its
+// second operand to the mantissa's 20 bits below a code step (and as far below the even steps under 2^-6) and cuts off: up with the
+// probability of the remainder.  Here 16 random bits, from the top.
+template <bool HIGH> __device__ __forceinline__ unsigned adamw_encode(unsigned codes, float y0, unsigned bits0, float y1, unsigned bits1) {
+  codes = (unsigned)__builtin_amdgcn_cvt_sr_fp8_f32(y0, (int)bits0, (int)codes, HIGH ? 2 : 0);
+  return (unsigned)__builtin_amdgcn_cvt_sr_fp8_f32(y1, (int)bits1, (int)codes, HIGH ? 3 : 1);
 }
 
-// the block's scale from its largest finite magnitude, as an exponent: the smallest k with amax <= 448 * 2^k, at least -126
-__device__ __forceinline__ int adamw_exponent(float amax) {
-  return max((int)((__float_as_uint(amax) + 0x1FFFFFu) >> 23) - 127 - 8, -126);
+// the block's scale from the bits of its largest finite magnitude, as an exponent: the smallest k with amax <= 448 * 2^k, at
+// least -126
+__device__ __forceinline__ int adamw_exponent(unsigned amax) {
+  return max((int)((amax + 0x1FFFFFu) >> 23) - 127 - 8, -126);
 }
 
-// Largest of a non-negative value over the wave, in every lane: DPP moves within and across the rows of 16, no LDS
-__device__ __forceinline__ float adamw_wave_max(float v) {
-#define ADAMW_DPP(ctrl) v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, false)))
+// Largest of the lanes' values (bits of magnitudes: they order as the magnitudes do): DPP moves within and across the rows of 16,
+// no LDS
+__device__ __forceinline__ unsigned adamw_wave_max(unsigned v) {
+#define ADAMW_DPP(ctrl) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xF, 0xF, false))
   ADAMW_DPP(0xB1);       // quad_perm [1,0,3,2]
   ADAMW_DPP(0x4E);       // quad_perm [2,3,0,1]
   ADAMW_DPP(0x124);      // row_ror:4
@@ -225,7 +230,7 @@ __device__ __forceinline__ float adamw_wave_max(float v) {
   ADAMW_DPP(0x142);      // row_bcast:15 -> the next row (rows 1, 3 hold two rows' maximum)
   ADAMW_DPP(0x143);      // row_bcast:31 -> rows 2, 3 (row 3 holds all)
 #undef ADAMW_DPP
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
 
 // One row of a tensor with 8-bit moments: codes and scales in, codes and scales out.  count: elements of this lane that exist.
@@ -240,36 +245,35 @@ __device__ __forceinline__ void adamw_row8(AdamwRow8& r, int count, unsigned pla
                        __builtin_amdgcn_cvt_f32_fp8(r.cm, 3)};
   const float ov[4] = {__builtin_amdgcn_cvt_f32_fp8(r.cv, 0), __builtin_amdgcn_cvt_f32_fp8(r.cv, 1), __builtin_amdgcn_cvt_f32_fp8(r.cv, 2),
                        __builtin_amdgcn_cvt_f32_fp8(r.cv, 3)};
-  float fm[4], fv[4], am = 0.f, av = 0.f;
+  float fm[4], fv[4];
+  unsigned am = 0, av = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const double g = (double)r.g[j] * coef;
     fm[j] = j < count ? (float)fma((double)om[j], ms, a.domb1 * g) : 0.f;
     fv[j] = j < count ? (float)fma((double)ov[j], vs, a.domb2 * g * g) : 0.f;
-    const float mag = fabsf(fm[j]);
-    am = fmaxf(am, mag <= 3.4028235e38f ? mag : 0.f);
-    av = fmaxf(av, fv[j] <= 3.4028235e38f ? fv[j] : 0.f);
+    const unsigned bm = __float_as_uint(fm[j]) & 0x7FFFFFFFu, bv = __float_as_uint(fv[j]) & 0x7FFFFFFFu;
+    am = max(am, bm < 0x7F800000u ? bm : 0u);
+    av = max(av, bv < 0x7F800000u ? bv : 0u);
   }
   am = adamw_wave_max(am);
   av = adamw_wave_max(av);
   const int em = adamw_exponent(am), ev = adamw_exponent(av);
   const float im = __uint_as_float((unsigned)(127 - em) << 23), iv = __uint_as_float((unsigned)(127 - ev) << 23);      // 2^-k
-  r.cm = r.cv = 0;
+  float ym[4], yv[4];
+  unsigned h[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const unsigned h = adamw_hash(place + j);
-    unsigned c = adamw_encode(fabsf(fm[j]) * im, h & 0xFFFFu);
-    if (!(fabsf(fm[j]) <= 3.4028235e38f)) c = 0x7F;
-    if (fm[j] < 0.f) c |= 0x80u;
-    r.cm |= c << (8 * j);
-    c = adamw_encode(fv[j] * iv, h >> 16);
-    if (fv[j] > 0.f) c = max(c, 1u);
-    if (!(fv[j] <= 3.4028235e38f)) c = 0x7F;
-    r.cv |= c << (8 * j);
+    h[j] = adamw_hash(place + j);
+    ym[j] = fmaf(fm[j], im, 0.f);                      // the sum makes -0 a +0
+    yv[j] = fv[j] > 0.f ? fmaxf(fv[j] * iv, 0x1p-9f) : fv[j];
     r.p[j] = adamw_update(r.p[j], fm[j], fv[j], keep, s, a.eps);
   }
-  r.ms = am > 0.f ? __uint_as_float((unsigned)(127 + em) << 23) : 0.f;
-  r.vs = av > 0.f ? __uint_as_float((unsigned)(127 + ev) << 23) : 0.f;
+  r.cm = adamw_encode<true>(adamw_encode<false>(0, ym[0], h[0] << 16, ym[1], h[1] << 16), ym[2], h[2] << 16, ym[3], h[3] << 16);
+  r.cv = adamw_encode<true>(adamw_encode<false>(0, yv[0], h[0] & 0xFFFF0000u, yv[1], h[1] & 0xFFFF0000u), yv[2], h[2] & 0xFFFF0000u,
+                            yv[3], h[3] & 0xFFFF0000u);
+  r.ms = am ? __uint_as_float((unsigned)(127 + em) << 23) : 0.f;
+  r.vs = av ? __uint_as_float((unsigned)(127 + ev) << 23) : 0.f;
 }
 
 struct Adamw8State {
