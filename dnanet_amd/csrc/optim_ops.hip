@@ -368,35 +368,60 @@ __global__ void adamw_hyper_kernel(float* hyper, long long* step, double beta1, 
 }
 
 // ---- global gradient norm: squares in fp64 (no overflow, no order that matters beyond 2^-53), fixed order ------------------
-__device__ __forceinline__ double adamw_block_sum(double v) {
-  __shared__ double red[ADAMW_THREADS / 64];
+template <int WAVES> __device__ __forceinline__ double adamw_block_sum(double v) {
+  __shared__ double red[WAVES];
 #pragma unroll
   for (int m = 32; m >= 1; m >>= 1) v += __shfl_xor(v, m);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   v = 0.0;
 #pragma unroll
-  for (int w = 0; w < ADAMW_THREADS / 64; ++w) v += red[w];
+  for (int w = 0; w < WAVES; ++w) v += red[w];
   return v;
+}
+template <typename G, int N> __device__ __forceinline__ double adamw_rows_norm(const AdamwEntry& e, long first, int rows) {
+  double sum = 0.0;
+  for (int row = threadIdx.x >> 6; row < rows; row += ADAMW_WAVES * N) {
+    const long i = first + (long)row * ADAMW_ROW + (threadIdx.x & 63) * 4;
+    float g[N][4];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      g[k][0] = g[k][1] = g[k][2] = g[k][3] = 0.f;
+      if (row + k * ADAMW_WAVES < rows) adamw_load<G>(e.g, i + (long)k * ADAMW_WAVES * ADAMW_ROW, 4, true, g[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum = fma((double)g[k][j], (double)g[k][j], sum);
+  }
+  return sum;
 }
 __global__ __launch_bounds__(ADAMW_THREADS) void grad_norm_kernel(AdamwList list, double* partial) {
   const AdamwEntry e = list.e[adamw_find(list, blockIdx.x)];
   const bool gb = e.flags & ADAMW_G_BF16, vec = e.flags & ADAMW_VECTOR;
   const long lo = (long)(blockIdx.x - e.block0) * ADAMW_CHUNK, hi = min(e.n, lo + ADAMW_CHUNK);
-  double sum = 0.0;
-  for (long i = lo + threadIdx.x * 4; i < hi; i += ADAMW_THREADS * 4) {
+  const int rows = vec ? (int)((hi - lo) / ADAMW_ROW) : 0;
+  double sum = gb ? adamw_rows_norm<__bf16, 4>(e, lo, rows) : adamw_rows_norm<float, 4>(e, lo, rows);
+  for (long i = lo + rows * ADAMW_ROW + threadIdx.x * 4; i < hi; i += ADAMW_THREADS * 4) {       // the rest, or an unaligned tensor
     float fg[4];
     adamw_load_any(e.g, gb, i, (int)min(4L, hi - i), vec, fg);
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum = fma((double)fg[j], (double)fg[j], sum);
   }
-  sum = adamw_block_sum(sum);
+  sum = adamw_block_sum<ADAMW_WAVES>(sum);
   if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
-__global__ __launch_bounds__(ADAMW_THREADS) void grad_norm_finalize_kernel(const double* partial, long count, float max_norm, float* out) {
+constexpr int ADAMW_JOIN = 1024;              // threads that add the partial sums, eight each at a time
+__global__ __launch_bounds__(ADAMW_JOIN) void grad_norm_finalize_kernel(const double* partial, long count, float max_norm, float* out) {
   double sum = 0.0;
-  for (long i = threadIdx.x; i < count; i += ADAMW_THREADS) sum += partial[i];
-  sum = adamw_block_sum(sum);
+  for (long i = threadIdx.x; i < count; i += ADAMW_JOIN * 8) {
+    double v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = i + k * ADAMW_JOIN < count ? partial[i + k * ADAMW_JOIN] : 0.0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += v[k];
+  }
+  sum = adamw_block_sum<ADAMW_JOIN / 64>(sum);
   if (threadIdx.x == 0) {
     const double norm = sqrt(sum), coef = (double)max_norm / (norm + 1e-6);
     out[0] = (float)norm;
@@ -509,7 +534,7 @@ int dn_grad_norm(const dn_adamw_tensor* tensors, int count, float max_norm, floa
     hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(ADAMW_THREADS), 0, st, list, partial + before);
   });
   if (rc) return rc;
-  hipLaunchKernelGGL(grad_norm_finalize_kernel, dim3(1), dim3(ADAMW_THREADS), 0, st, partial, need / (long)sizeof(double) - 1, max_norm, out);
+  hipLaunchKernelGGL(grad_norm_finalize_kernel, dim3(1), dim3(ADAMW_JOIN), 0, st, partial, need / (long)sizeof(double) - 1, max_norm, out);
   DN_LAUNCH_CHECK();
   return DN_OK;
 }
