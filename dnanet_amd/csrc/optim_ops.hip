@@ -25,7 +25,7 @@ namespace {
 
 constexpr int ADAMW_MAX = 96;                 // tensors of a launch: their records fill the 4-KiB kernel argument segment
 constexpr int ADAMW_THREADS = 256;
-constexpr int ADAMW_CHUNK = 4096;             // elements of a block: a multiple of the 256-element state blocks
+constexpr int ADAMW_CHUNK = 2048;             // elements of a block: a multiple of the 256-element state blocks
 constexpr unsigned ADAMW_P_BF16 = 1, ADAMW_G_BF16 = 2, ADAMW_VECTOR = 4;
 
 struct AdamwEntry {                           // 40 bytes
@@ -126,8 +126,8 @@ __device__ __forceinline__ float adamw_update(float p, float m, float v, float k
   return fmaf(-s.step_size * m, __builtin_amdgcn_rcpf(denom), p * keep);
 }
 
-// A row is 256 elements, four of each lane of a wave; a block's waves take the rows of its chunk in turn.
-constexpr int ADAMW_ROW = 256, ADAMW_WAVES = ADAMW_THREADS / 64;
+// A row is 256 elements, four of each lane of a wave; a wave's rows are all in flight at once.
+constexpr int ADAMW_ROW = 256, ADAMW_WAVES = ADAMW_THREADS / 64, ADAMW_ROWS = ADAMW_CHUNK / ADAMW_ROW / ADAMW_WAVES;
 
 struct AdamwRow32 { float p[4], g[4], m[4], v[4]; };
 __device__ __forceinline__ void adamw_row32(AdamwRow32& r, const AdamwArgs& a, const AdamwScalars& s, float keep) {
@@ -139,36 +139,35 @@ __device__ __forceinline__ void adamw_row32(AdamwRow32& r, const AdamwArgs& a, c
     r.p[j] = adamw_update(r.p[j], r.m[j], r.v[j], keep, s, a.eps);
   }
 }
-// `rows` whole rows of an aligned tensor from element i of lane 0 on, N at a time in flight
-template <typename P, typename G, int N>
+// `rows` whole rows of an aligned tensor from element `first` on
+template <typename P, typename G>
 __device__ __forceinline__ void adamw_rows32(const AdamwEntry& e, long first, int rows, float* m, float* v, const AdamwArgs& a,
                                              const AdamwScalars& s, float keep) {
-  for (int row = threadIdx.x >> 6; row < rows; row += ADAMW_WAVES * N) {
-    AdamwRow32 r[N];
-    const long i = first + (long)row * ADAMW_ROW + (threadIdx.x & 63) * 4;
+  const int row = threadIdx.x >> 6;
+  AdamwRow32 r[ADAMW_ROWS];
+  const long i = first + (long)row * ADAMW_ROW + (threadIdx.x & 63) * 4;
 #pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (row + k * ADAMW_WAVES < rows) {
-        const long at = i + (long)k * ADAMW_WAVES * ADAMW_ROW;
-        adamw_load<P>(e.p, at, 4, true, r[k].p);
-        adamw_load<G>(e.g, at, 4, true, r[k].g);
-        adamw_load<float>(m, at, 4, true, r[k].m);
-        adamw_load<float>(v, at, 4, true, r[k].v);
-      }
+  for (int k = 0; k < ADAMW_ROWS; ++k)
+    if (row + k * ADAMW_WAVES < rows) {
+      const long at = i + (long)k * ADAMW_WAVES * ADAMW_ROW;
+      adamw_load<P>(e.p, at, 4, true, r[k].p);
+      adamw_load<G>(e.g, at, 4, true, r[k].g);
+      adamw_load<float>(m, at, 4, true, r[k].m);
+      adamw_load<float>(v, at, 4, true, r[k].v);
+    }
 #pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (row + k * ADAMW_WAVES < rows) {
-        const long at = i + (long)k * ADAMW_WAVES * ADAMW_ROW;
-        adamw_row32(r[k], a, s, keep);
-        adamw_store<P>(e.p, at, 4, true, r[k].p);
-        adamw_store<float>(m, at, 4, true, r[k].m);
-        adamw_store<float>(v, at, 4, true, r[k].v);
-        if (a.zero_grad) {
-          const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-          adamw_store<G>(e.g, at, 4, true, zero);
-        }
+  for (int k = 0; k < ADAMW_ROWS; ++k)
+    if (row + k * ADAMW_WAVES < rows) {
+      const long at = i + (long)k * ADAMW_WAVES * ADAMW_ROW;
+      adamw_row32(r[k], a, s, keep);
+      adamw_store<P>(e.p, at, 4, true, r[k].p);
+      adamw_store<float>(m, at, 4, true, r[k].m);
+      adamw_store<float>(v, at, 4, true, r[k].v);
+      if (a.zero_grad) {
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        adamw_store<G>(e.g, at, 4, true, zero);
       }
-  }
+    }
 }
 
 __global__ __launch_bounds__(ADAMW_THREADS) void adamw_kernel(AdamwList list, float* exp_avg, float* exp_avg_sq, AdamwArgs a) {
@@ -181,11 +180,11 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw_kernel(AdamwList list, fl
   const bool pb = e.flags & ADAMW_P_BF16, gb = e.flags & ADAMW_G_BF16, vec = e.flags & ADAMW_VECTOR;
   const int rows = vec ? (int)((hi - lo) / ADAMW_ROW) : 0;
   if (pb) {
-    if (gb) adamw_rows32<__bf16, __bf16, 2>(e, lo, rows, m, v, a, s, keep);
-    else adamw_rows32<__bf16, float, 2>(e, lo, rows, m, v, a, s, keep);
+    if (gb) adamw_rows32<__bf16, __bf16>(e, lo, rows, m, v, a, s, keep);
+    else adamw_rows32<__bf16, float>(e, lo, rows, m, v, a, s, keep);
   } else {
-    if (gb) adamw_rows32<float, __bf16, 2>(e, lo, rows, m, v, a, s, keep);
-    else adamw_rows32<float, float, 2>(e, lo, rows, m, v, a, s, keep);
+    if (gb) adamw_rows32<float, __bf16>(e, lo, rows, m, v, a, s, keep);
+    else adamw_rows32<float, float>(e, lo, rows, m, v, a, s, keep);
   }
   for (long i = lo + rows * ADAMW_ROW + threadIdx.x * 4; i < hi; i += ADAMW_THREADS * 4) {       // the rest, or an unaligned tensor
     const int count = (int)min(4L, hi - i);
@@ -280,38 +279,37 @@ struct Adamw8State {
   unsigned char *m, *v;
   float *ms, *vs;
 };
-template <typename P, typename G, int N>
+template <typename P, typename G>
 __device__ __forceinline__ void adamw_rows8(const AdamwEntry& e, long first, int rows, const Adamw8State& o, unsigned key, const AdamwArgs& a,
                                             const AdamwScalars& s, float keep) {
   const int lane = threadIdx.x & 63;
-  for (int row = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); row < rows; row += ADAMW_WAVES * N) {
-    AdamwRow8 r[N];
+  const int row = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  AdamwRow8 r[ADAMW_ROWS];
 #pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (row + k * ADAMW_WAVES < rows) {
-        const long base = first + (long)(row + k * ADAMW_WAVES) * ADAMW_ROW, at = base + lane * 4;
-        adamw_load<P>(e.p, at, 4, true, r[k].p);
-        adamw_load<G>(e.g, at, 4, true, r[k].g);
-        r[k].cm = *(const unsigned*)(o.m + at);
-        r[k].cv = *(const unsigned*)(o.v + at);
-        r[k].ms = o.ms[base >> 8];
-        r[k].vs = o.vs[base >> 8];
-      }
+  for (int k = 0; k < ADAMW_ROWS; ++k)
+    if (row + k * ADAMW_WAVES < rows) {
+      const long base = first + (long)(row + k * ADAMW_WAVES) * ADAMW_ROW, at = base + lane * 4;
+      adamw_load<P>(e.p, at, 4, true, r[k].p);
+      adamw_load<G>(e.g, at, 4, true, r[k].g);
+      r[k].cm = *(const unsigned*)(o.m + at);
+      r[k].cv = *(const unsigned*)(o.v + at);
+      r[k].ms = o.ms[base >> 8];
+      r[k].vs = o.vs[base >> 8];
+    }
 #pragma unroll
-    for (int k = 0; k < N; ++k)
-      if (row + k * ADAMW_WAVES < rows) {
-        const long base = first + (long)(row + k * ADAMW_WAVES) * ADAMW_ROW, at = base + lane * 4;
-        adamw_row8(r[k], 4, (unsigned)at + key, a, s, keep);
-        adamw_store<P>(e.p, at, 4, true, r[k].p);
-        *(unsigned*)(o.m + at) = r[k].cm;
-        *(unsigned*)(o.v + at) = r[k].cv;
-        if (lane == 0) { o.ms[base >> 8] = r[k].ms; o.vs[base >> 8] = r[k].vs; }
-        if (a.zero_grad) {
-          const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-          adamw_store<G>(e.g, at, 4, true, zero);
-        }
+  for (int k = 0; k < ADAMW_ROWS; ++k)
+    if (row + k * ADAMW_WAVES < rows) {
+      const long base = first + (long)(row + k * ADAMW_WAVES) * ADAMW_ROW, at = base + lane * 4;
+      adamw_row8(r[k], 4, (unsigned)at + key, a, s, keep);
+      adamw_store<P>(e.p, at, 4, true, r[k].p);
+      *(unsigned*)(o.m + at) = r[k].cm;
+      *(unsigned*)(o.v + at) = r[k].cv;
+      if (lane == 0) { o.ms[base >> 8] = r[k].ms; o.vs[base >> 8] = r[k].vs; }
+      if (a.zero_grad) {
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        adamw_store<G>(e.g, at, 4, true, zero);
       }
-  }
+    }
 }
 
 __global__ __launch_bounds__(ADAMW_THREADS) void adamw8_kernel(AdamwList list, unsigned char* exp_avg, unsigned char* exp_avg_sq,
@@ -325,11 +323,11 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw8_kernel(AdamwList list, u
   const bool pb = e.flags & ADAMW_P_BF16, gb = e.flags & ADAMW_G_BF16, vec = e.flags & ADAMW_VECTOR;
   const int rows = vec ? (int)((hi - lo) / ADAMW_ROW) : 0;
   if (pb) {
-    if (gb) adamw_rows8<__bf16, __bf16, 2>(e, lo, rows, o, key, a, s, keep);
-    else adamw_rows8<__bf16, float, 2>(e, lo, rows, o, key, a, s, keep);
+    if (gb) adamw_rows8<__bf16, __bf16>(e, lo, rows, o, key, a, s, keep);
+    else adamw_rows8<__bf16, float>(e, lo, rows, o, key, a, s, keep);
   } else {
-    if (gb) adamw_rows8<float, __bf16, 2>(e, lo, rows, o, key, a, s, keep);
-    else adamw_rows8<float, float, 2>(e, lo, rows, o, key, a, s, keep);
+    if (gb) adamw_rows8<float, __bf16>(e, lo, rows, o, key, a, s, keep);
+    else adamw_rows8<float, float>(e, lo, rows, o, key, a, s, keep);
   }
   const int lane = threadIdx.x & 63;
   for (long base = lo + (rows + (threadIdx.x >> 6)) * ADAMW_ROW; base < hi; base += ADAMW_WAVES * ADAMW_ROW) {      // the rest, or an unaligned tensor
@@ -379,29 +377,29 @@ template <int WAVES> __device__ __forceinline__ double adamw_block_sum(double v)
   for (int w = 0; w < WAVES; ++w) v += red[w];
   return v;
 }
-template <typename G, int N> __device__ __forceinline__ double adamw_rows_norm(const AdamwEntry& e, long first, int rows) {
-  double sum = 0.0;
-  for (int row = threadIdx.x >> 6; row < rows; row += ADAMW_WAVES * N) {
-    const long i = first + (long)row * ADAMW_ROW + (threadIdx.x & 63) * 4;
-    float g[N][4];
+constexpr int NORM_CHUNK = 8192, NORM_ROWS = NORM_CHUNK / ADAMW_ROW / ADAMW_WAVES;      // fewer partial sums to join
+template <typename G> __device__ __forceinline__ double adamw_rows_norm(const AdamwEntry& e, long first, int rows) {
+  const int row = threadIdx.x >> 6;
+  const long i = first + (long)row * ADAMW_ROW + (threadIdx.x & 63) * 4;
+  float g[NORM_ROWS][4];
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      g[k][0] = g[k][1] = g[k][2] = g[k][3] = 0.f;
-      if (row + k * ADAMW_WAVES < rows) adamw_load<G>(e.g, i + (long)k * ADAMW_WAVES * ADAMW_ROW, 4, true, g[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sum = fma((double)g[k][j], (double)g[k][j], sum);
+  for (int k = 0; k < NORM_ROWS; ++k) {
+    g[k][0] = g[k][1] = g[k][2] = g[k][3] = 0.f;
+    if (row + k * ADAMW_WAVES < rows) adamw_load<G>(e.g, i + (long)k * ADAMW_WAVES * ADAMW_ROW, 4, true, g[k]);
   }
+  double sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < NORM_ROWS; ++k)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum = fma((double)g[k][j], (double)g[k][j], sum);
   return sum;
 }
 __global__ __launch_bounds__(ADAMW_THREADS) void grad_norm_kernel(AdamwList list, double* partial) {
   const AdamwEntry e = list.e[adamw_find(list, blockIdx.x)];
   const bool gb = e.flags & ADAMW_G_BF16, vec = e.flags & ADAMW_VECTOR;
-  const long lo = (long)(blockIdx.x - e.block0) * ADAMW_CHUNK, hi = min(e.n, lo + ADAMW_CHUNK);
+  const long lo = (long)(blockIdx.x - e.block0) * NORM_CHUNK, hi = min(e.n, lo + NORM_CHUNK);
   const int rows = vec ? (int)((hi - lo) / ADAMW_ROW) : 0;
-  double sum = gb ? adamw_rows_norm<__bf16, 4>(e, lo, rows) : adamw_rows_norm<float, 4>(e, lo, rows);
+  double sum = gb ? adamw_rows_norm<__bf16>(e, lo, rows) : adamw_rows_norm<float>(e, lo, rows);
   for (long i = lo + rows * ADAMW_ROW + threadIdx.x * 4; i < hi; i += ADAMW_THREADS * 4) {       // the rest, or an unaligned tensor
     float fg[4];
     adamw_load_any(e.g, gb, i, (int)min(4L, hi - i), vec, fg);
@@ -429,7 +427,7 @@ __global__ __launch_bounds__(ADAMW_JOIN) void grad_norm_finalize_kernel(const do
   }
 }
 
-long adamw_blocks(long n) { return (n + ADAMW_CHUNK - 1) / ADAMW_CHUNK; }
+long adamw_blocks(long n, int chunk) { return (n + chunk - 1) / chunk; }
 
 int adamw_check(const char* name, const dn_adamw_tensor* t, int count, bool state) {
   DN_CHECK_ARG(count >= 0 && (t || count == 0), "%s: null tensor list", name);
@@ -448,12 +446,12 @@ int adamw_check(const char* name, const dn_adamw_tensor* t, int count, bool stat
 }
 
 // The next launch's tensors from t[*first] on (empty ones are left out); returns its blocks, 0 when none is left
-long adamw_fill(const dn_adamw_tensor* t, int count, int* first, AdamwList* l) {
+long adamw_fill(const dn_adamw_tensor* t, int count, int chunk, int* first, AdamwList* l) {
   long blocks = 0;
   l->count = 0;
   while (*first < count && l->count < ADAMW_MAX) {
     const dn_adamw_tensor& x = t[*first];
-    const long more = adamw_blocks(x.n);
+    const long more = adamw_blocks(x.n, chunk);
     if (blocks && blocks + more >= (1L << 31)) break;
     if (x.n > 0) {
       AdamwEntry& e = l->e[l->count];
@@ -469,12 +467,12 @@ long adamw_fill(const dn_adamw_tensor* t, int count, int* first, AdamwList* l) {
   return blocks;
 }
 
-// launches `kernel(list, ...)` over all tensors
-template <typename F> int adamw_each_launch(const dn_adamw_tensor* t, int count, F launch) {
+// launch(list, blocks, blocks before) over all tensors, `chunk` elements a block
+template <typename F> int adamw_each_launch(const dn_adamw_tensor* t, int count, int chunk, F launch) {
   AdamwList list;
   long before = 0;
   for (int first = 0; first < count;) {
-    const long blocks = adamw_fill(t, count, &first, &list);
+    const long blocks = adamw_fill(t, count, chunk, &first, &list);
     if (!blocks) break;
     launch(list, (unsigned)blocks, before);
     DN_LAUNCH_CHECK();
@@ -485,7 +483,7 @@ template <typename F> int adamw_each_launch(const dn_adamw_tensor* t, int count,
 
 int adamw_run(const dn_adamw_tensor* tensors, int count, void* exp_avg, void* exp_avg_sq, float* m_scale, float* v_scale,
               int state_bits, const AdamwArgs& a, hipStream_t st) {
-  return adamw_each_launch(tensors, count, [&](const AdamwList& list, unsigned blocks, long) {
+  return adamw_each_launch(tensors, count, ADAMW_CHUNK, [&](const AdamwList& list, unsigned blocks, long) {
     if (state_bits == 8)
       hipLaunchKernelGGL(adamw8_kernel, dim3(blocks), dim3(ADAMW_THREADS), 0, st, list, (unsigned char*)exp_avg, (unsigned char*)exp_avg_sq,
                          m_scale, v_scale, a);
@@ -518,7 +516,7 @@ extern "C" {
 long dn_grad_norm_workspace_bytes(const dn_adamw_tensor* tensors, int count) {
   if (adamw_check("dn_grad_norm_workspace_bytes", tensors, count, false)) return -1;
   long blocks = 1;
-  for (int i = 0; i < count; ++i) blocks += adamw_blocks(tensors[i].n);
+  for (int i = 0; i < count; ++i) blocks += adamw_blocks(tensors[i].n, NORM_CHUNK);
   return blocks * (long)sizeof(double);
 }
 
@@ -530,7 +528,7 @@ int dn_grad_norm(const dn_adamw_tensor* tensors, int count, float max_norm, floa
                "dn_grad_norm: workspace of %ld bytes, %ld needed (8-byte aligned)", workspace_bytes, need);
   double* partial = (double*)workspace;
   const hipStream_t st = (hipStream_t)stream;
-  const int rc = adamw_each_launch(tensors, count, [&](const AdamwList& list, unsigned blocks, long before) {
+  const int rc = adamw_each_launch(tensors, count, NORM_CHUNK, [&](const AdamwList& list, unsigned blocks, long before) {
     hipLaunchKernelGGL(grad_norm_kernel, dim3(blocks), dim3(ADAMW_THREADS), 0, st, list, partial + before);
   });
   if (rc) return rc;
