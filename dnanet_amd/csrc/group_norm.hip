@@ -480,7 +480,9 @@ __device__ __forceinline__ bool gnf_place(const GnFused& f, unsigned* lds2, GnPl
     if (!u.alone) {
       unsigned* next = f.ctrl + (3 + 2 * u.shard) * GNF_LINE;
       place = gnf_count(next);
-      if (place == (unsigned)gn_div(f.d_shards, (int)gridDim.x) - 1) gnf_reset(next);                // the shard's last block to start
+      const unsigned blocks = (unsigned)gn_div(f.d_shards, (int)gridDim.x);                         // of this shard
+      if (place == blocks - 1) gnf_reset(next);                                                     // the last to start
+      if (place >= blocks) place = blocks;                                                          // a workspace that was not zeroed
       epoch = __hip_atomic_load(f.ctrl, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     lds2[0] = place;
@@ -490,7 +492,7 @@ __device__ __forceinline__ bool gnf_place(const GnFused& f, unsigned* lds2, GnPl
   __syncthreads();
   u.tag = (unsigned)__builtin_amdgcn_readfirstlane(lds2[1]) % 0xFFFFFFFFu + 1;         // never 0, what the workspace is filled with at first
   gnf_locate(f, u, __builtin_amdgcn_readfirstlane(lds2[0]));                           // scalar from here on
-  return u.cluster < (long)f.images * f.nsets && u.plane < f.s.P;
+  return u.cluster < (long)f.images * f.nsets && u.plane < f.s.P && (u.alone || u.place < (unsigned)gn_div(f.d_shards, (int)gridDim.x));
 }
 
 // Sums over the wave's 32 lanes of equal record half, of four channels at a time (h: which four of the thread's half record):
@@ -1019,6 +1021,19 @@ int gn_tensor(const char* name, const char* which, dn_tensor t, const GnShape& s
                t.plane0 + s.P, which, t.planes_total);
   return DN_OK;
 }
+// Whether tensors a and b share memory without being the same planes (the same planes: in place).
+bool gn_mixed_up(dn_tensor a, dn_tensor b, const GnShape& s) {
+  const long plane = s.npieces * 16L;
+  if (a.base == b.base && a.planes_total == b.planes_total) {
+    const int apart = a.plane0 > b.plane0 ? a.plane0 - b.plane0 : b.plane0 - a.plane0;
+    return apart != 0 && apart < s.P;
+  }
+  const char *a0 = (const char*)a.base + a.plane0 * plane, *b0 = (const char*)b.base + b.plane0 * plane;
+  return a0 < b0 + ((s.N - 1L) * b.planes_total + s.P) * plane && b0 < a0 + ((s.N - 1L) * a.planes_total + s.P) * plane;
+}
+bool gn_same(dn_tensor a, dn_tensor b) { return a.base == b.base && a.planes_total == b.planes_total && a.plane0 == b.plane0; }
+// the three-launch form's blocks: a launch holds less than 2^32 threads
+bool gn_launches(const GnShape& s) { return std::max((long)s.N * s.P * s.nseg, (long)s.N * s.G) * GN_THREADS < 1L << 32; }
 long gn_part_bytes(const GnShape& s, int dtype) {
   return (long)s.N * s.P * s.nseg * (dtype == DN_BF16 ? 16 : 8) * (long)sizeof(float2);
 }
@@ -1170,8 +1185,11 @@ int dn_group_norm_act(dn_tensor x, dn_tensor a, int N, int H, int W, int groups,
   DN_CHECK_ARG(gamma && beta && mean && rstd && scale && shift, "dn_group_norm_act: null vector");
   DN_CHECK_ARG(eps >= 1e-30f && eps <= 1e30f, "dn_group_norm_act: eps must be within 1e-30 and 1e30");
   DN_CHECK_ARG(act >= DN_ACT_NONE && act <= DN_ACT_SILU, "dn_group_norm_act: bad activation %d", act);
+  GnFused f;
+  DN_CHECK_ARG(gn_fused_plan(s, dtype, GNF_R, &f) || gn_launches(s), "dn_group_norm_act: too many images x planes");
   DN_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= gn_workspace(s, dtype),
                "dn_group_norm_act: workspace of %ld bytes, %ld needed (16-byte aligned)", workspace_bytes, gn_workspace(s, dtype));
+  DN_CHECK_ARG(!gn_mixed_up(a, x, s), "dn_group_norm_act: a overlaps x and is not x");
 #define GN_CALL(T, A) (gn_forward_launch<T, A>(x, a, s, gamma, beta, eps, mean, rstd, scale, shift, workspace, dtype, (hipStream_t)stream))
   GN_DISPATCH(dtype, act, GN_CALL)
 #undef GN_CALL
@@ -1191,8 +1209,13 @@ int dn_group_norm_act_backward(dn_tensor g, dn_tensor x, dn_tensor dx, int N, in
     return rc;
   DN_CHECK_ARG(gamma && mean && rstd && scale && shift && dgamma && dbeta, "dn_group_norm_act_backward: null vector");
   DN_CHECK_ARG(act >= DN_ACT_NONE && act <= DN_ACT_SILU, "dn_group_norm_act_backward: bad activation %d", act);
+  GnFused f;
+  DN_CHECK_ARG(gn_fused_plan(s, dtype, GNF_R_BWD, &f) || gn_launches(s), "dn_group_norm_act_backward: too many images x planes");
   DN_CHECK_ARG(workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= gn_workspace(s, dtype),
                "dn_group_norm_act_backward: workspace of %ld bytes, %ld needed (16-byte aligned)", workspace_bytes, gn_workspace(s, dtype));
+  DN_CHECK_ARG(!gn_mixed_up(dx, g, s), "dn_group_norm_act_backward: dx overlaps g and is not g");
+  DN_CHECK_ARG(!gn_mixed_up(dx, x, s) && !gn_same(dx, x), "dn_group_norm_act_backward: dx overlaps x");
+  DN_CHECK_ARG(dgamma + s.C <= dbeta || dbeta + s.C <= dgamma, "dn_group_norm_act_backward: dgamma and dbeta overlap");
 #define GN_CALL(T, A) (gn_backward_launch<T, A>(g, x, dx, s, gamma, mean, rstd, scale, shift, dgamma, dbeta, workspace, dtype, (hipStream_t)stream))
   GN_DISPATCH(dtype, act, GN_CALL)
 #undef GN_CALL

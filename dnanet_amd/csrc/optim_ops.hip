@@ -377,7 +377,7 @@ template <int WAVES> __device__ __forceinline__ double adamw_block_sum(double v)
   for (int w = 0; w < WAVES; ++w) v += red[w];
   return v;
 }
-constexpr int NORM_CHUNK = 8192, NORM_ROWS = NORM_CHUNK / ADAMW_ROW / ADAMW_WAVES;      // fewer partial sums to join
+constexpr int NORM_CHUNK = 4096, NORM_ROWS = NORM_CHUNK / ADAMW_ROW / ADAMW_WAVES;      // fewer partial sums to join
 template <typename G> __device__ __forceinline__ double adamw_rows_norm(const AdamwEntry& e, long first, int rows) {
   const int row = threadIdx.x >> 6;
   const long i = first + (long)row * ADAMW_ROW + (threadIdx.x & 63) * 4;
@@ -432,7 +432,7 @@ long adamw_blocks(long n, int chunk) { return (n + chunk - 1) / chunk; }
 int adamw_check(const char* name, const dn_adamw_tensor* t, int count, bool state) {
   DN_CHECK_ARG(count >= 0 && (t || count == 0), "%s: null tensor list", name);
   for (int i = 0; i < count; ++i) {
-    DN_CHECK_ARG(t[i].n >= 0 && t[i].n <= (1L << 40), "%s: tensor %d has %ld elements", name, i, t[i].n);
+    DN_CHECK_ARG(t[i].n >= 0 && t[i].n <= (1L << 34), "%s: tensor %d has %ld elements", name, i, t[i].n);
     if (t[i].n == 0) continue;
     DN_CHECK_ARG(t[i].grad && (t[i].param || !state), "%s: tensor %d: null pointer", name, i);
     DN_CHECK_ARG((t[i].param_dtype == DN_F32 || t[i].param_dtype == DN_BF16) && (t[i].grad_dtype == DN_F32 || t[i].grad_dtype == DN_BF16),
@@ -452,7 +452,7 @@ long adamw_fill(const dn_adamw_tensor* t, int count, int chunk, int* first, Adam
   while (*first < count && l->count < ADAMW_MAX) {
     const dn_adamw_tensor& x = t[*first];
     const long more = adamw_blocks(x.n, chunk);
-    if (blocks && blocks + more >= (1L << 31)) break;
+    if (blocks && blocks + more >= 1L << 24) break;            // a launch holds less than 2^32 threads
     if (x.n > 0) {
       AdamwEntry& e = l->e[l->count];
       e.p = x.param; e.g = x.grad; e.n = x.n; e.state = (unsigned)(x.state / 256); e.decay = x.weight_decay; e.block0 = (unsigned)blocks;

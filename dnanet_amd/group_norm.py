@@ -116,6 +116,12 @@ def _vector(t: torch.Tensor, shape, device, what: str) -> int:
     return t.data_ptr()
 
 
+def _given_workspace(ws: torch.Tensor, device) -> torch.Tensor:
+    if ws.dtype != torch.uint8 or ws.device != device or not ws.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous uint8 tensor on {device}, got {ws.dtype} on {ws.device}")
+    return ws
+
+
 def _need(n: int, channels: int, h: int, w: int, groups: int, dtype: int) -> int:
     nbytes = hip.lib.dn_group_norm_workspace_bytes(n, channels, h, w, groups, dtype)
     if nbytes < 0:
@@ -145,7 +151,7 @@ def group_norm_act(x: DnTensor, gamma: torch.Tensor, beta: torch.Tensor, groups:
     vectors = stats._pointers(src.n, c, groups, dev)
     with _on(dev):
         stream = hip.raw_stream(dev)
-        ws = _workspace(dev, stream, need) if workspace is None else workspace
+        ws = _workspace(dev, stream, need) if workspace is None else _given_workspace(workspace, dev)
         hip.check(hip.lib.dn_group_norm_act(x, out, src.n, src.h, src.w, groups, g, b, eps, act, *vectors, ws.data_ptr(), ws.numel(),
                                             src.dtype, stream))
     stats.groups, stats.activation = groups, activation
@@ -178,7 +184,7 @@ def group_norm_act_backward(g: DnTensor, x: DnTensor, gamma: torch.Tensor, stats
     dg, db = _vector(dgamma, (c,), dev, "dgamma"), _vector(dbeta, (c,), dev, "dbeta")
     with _on(dev):
         stream = hip.raw_stream(dev)
-        ws = _workspace(dev, stream, need) if workspace is None else workspace
+        ws = _workspace(dev, stream, need) if workspace is None else _given_workspace(workspace, dev)
         hip.check(hip.lib.dn_group_norm_act_backward(g, x, out, src.n, src.h, src.w, groups, ga, *vectors, parse_activation(stats.activation),
                                                      dg, db, ws.data_ptr(), ws.numel(), src.dtype, stream))
     return dst, dgamma, dbeta

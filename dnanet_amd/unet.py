@@ -363,11 +363,15 @@ class HipUNet(ParameterTree):
                                       hip.ptr(logits), hip.ptr(probs), n, h, w, dt, hip.stream_ptr()))
 
     def _group_norm_workspace(self, channels: int, n: int, h: int, w: int) -> torch.Tensor:
-        """The model's group-norm workspace (zeroed when allocated; the passes of one model follow each other)."""
+        """The model's group-norm workspace (zeroed when allocated; the passes of one model follow each other).  A pass that
+        someone captures into a graph of theirs gets one inside the graph: the zeroing of the model's own would be captured
+        and not done, and a later, larger batch would free it under the graph."""
         ws = self._workspace()
         need = hip.lib.dn_group_norm_workspace_bytes(n, channels, h, w, self.num_groups, self.dtype)
         if need < 0:
             hip.check(1)
+        if self._arena_override is None and torch.cuda.is_current_stream_capturing():
+            return torch.zeros(need, dtype=torch.uint8, device=self.device)
         if ws.get("group_norm") is None or ws["group_norm"].numel() < need:
             ws["group_norm"] = torch.zeros(need, dtype=torch.uint8, device=self.device)
         return ws["group_norm"]
@@ -1061,6 +1065,9 @@ class GraphedTrainStep:
         self._lr_dev, self._step_expected = None, None
         model.train()
         model._workspace()
+        if model.norm == "group":                          # as large as any of the net's units needs it, and zeroed now
+            for u in model.conv_units:
+                model._group_norm_workspace(u.cout, x.shape[0], x.shape[2], x.shape[3] >> u.level)
         model._build_train_cache()                         # job table and image buffers exist before the capture ...
         model._train_cache_version = None                  # ... and the re-packing launch itself is part of the graph
         self.graph = torch.cuda.CUDAGraph()

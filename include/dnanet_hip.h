@@ -257,7 +257,7 @@ int dn_bn_train_backward_apply_totals(dn_tensor g, dn_tensor y, const float* sca
  * torch.nn.functional.group_norm(x, groups, gamma, beta, eps) followed by the activation, per image and group over the
  * group's channels and H x W.  gamma / beta: [C]; mean / rstd: [N][groups]; scale / shift: [N][dn_channel_pad(C)], zero past
  * C: gamma * rstd and beta - mean * scale, kept for the backward pass.  C is a multiple of groups (groups need not fill
- * records), H * W <= 2^25, 1e-30 <= eps <= 1e30.  a may be x.  N = 0 returns without a launch.
+ * records), H * W <= 2^25, 1e-30 <= eps <= 1e30.  a may be x, and shares no memory with it otherwise.  N = 0 returns without a launch.
  * workspace: dn_group_norm_workspace_bytes (-1: refused sizes), 16-byte aligned; zero-filled by the caller before its first
  * use, left for the next call as each call needs it.  It may serve any sizes it is large enough for, one call at a time:
  * calls that overlap on the GPU need workspaces of their own. */
@@ -267,7 +267,7 @@ int dn_bn_train_backward_apply_totals(dn_tensor g, dn_tensor y, const float* sca
 long dn_group_norm_workspace_bytes(int N, int C, int H, int W, int groups, int dtype);
 int dn_group_norm_act(dn_tensor x, dn_tensor a, int N, int H, int W, int groups, const float* gamma, const float* beta, float eps, int act,
                       float* mean, float* rstd, float* scale, float* shift, void* workspace, long workspace_bytes, int dtype, void* stream);
-/* Its backward: g = dL/da in, dx = dL/dx out (dx may be g; not x), dgamma / dbeta [C] overwritten.  mean / rstd / scale / shift as
+/* Its backward: g = dL/da in, dx = dL/dx out (dx may be g; it shares no memory with x), dgamma / dbeta [C] overwritten.  mean / rstd / scale / shift as
  * the forward call saved them; the activation's derivative is taken at x * scale + shift. */
 int dn_group_norm_act_backward(dn_tensor g, dn_tensor x, dn_tensor dx, int N, int H, int W, int groups, const float* gamma,
                                const float* mean, const float* rstd, const float* scale, const float* shift, int act, float* dgamma,
@@ -336,7 +336,7 @@ int dn_adam_step_graph(float* params, float* grads, float* exp_avg, float* exp_a
 typedef struct dn_adamw_tensor {
   void* param;           /* contiguous, param_dtype */
   void* grad;            /* contiguous, grad_dtype */
-  long n;                /* elements; 0: left out */
+  long n;                /* elements, up to 2^34; 0: left out */
   long state;            /* first element in the moment buffers, a multiple of 256 */
   float weight_decay;
   int param_dtype, grad_dtype;   /* DN_DTYPE_F32 | DN_DTYPE_BF16 */

@@ -396,3 +396,40 @@ def test_refusals(gpu_device):
     with pytest.raises(ValueError, match="contiguous"):
         opt.step()
     assert opt.step_count == 0
+
+
+def test_8_bit_signed_zeros_and_denormals(gpu_device):
+    """Gradients of both zeros, fp32 denormals and magnitudes whose moments round to zero: codes and scales bit by bit, no code of
+    a negative zero from a zero."""
+    from dnanet_amd.optim import HipAdamW
+    gen = torch.Generator().manual_seed(12)
+    n = 2048 + 100
+    p = torch.randn(n, generator=gen).cuda()
+    opt = HipAdamW([p], state_bits=8, seed=3)
+    p.grad = torch.empty(n).cuda()
+    state = [(torch.zeros(n, dtype=torch.float64), torch.zeros((n + 255) // 256, dtype=torch.float64)) for _ in range(2)]
+    size = torch.tensor([0.0, -0.0, 1e-42, -1e-42, 1e-30, -1e-30, 1.0, -1.0, 1e-3, -1e-4])
+    for t in range(1, 4):
+        g = size[torch.randint(len(size), (n,), generator=gen)]
+        g[:256], g[256:512], g[512:768] = g[:256].sign() * 1e-40, -0.0, g[512:768].sign() * 1e-36
+        p.grad.copy_(g)
+        opt.step()
+        _, state, _ = step8(torch.zeros(n, dtype=torch.float64), p.grad.double().cpu(), state, t, 0, 3)
+        for (q, s), codes, scales in zip(state, (opt.exp_avg, opt.exp_avg_sq), (opt.exp_avg_scale, opt.exp_avg_sq_scale)):
+            assert torch.equal(scales.double().cpu(), s) and torch.equal(codes[:n].float().double().cpu(), q)
+    assert not opt.exp_avg.view(torch.uint8)[256:512].any() and not opt.exp_avg_sq.view(torch.uint8)[256:512].any()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_denormal_second_moments_without_eps(gpu_device, bits):
+    """eps = 0 and gradients of 1e-18: the second moment, 1e-39 and up, is an fp32 denormal.  The first step is lr * sign(g), off by
+    half of v's error, two roundings to 2^-150 of at least 1e-39, and 16 roundings of the quotient."""
+    from dnanet_amd.optim import HipAdamW
+    gen = torch.Generator().manual_seed(5)
+    p = torch.zeros(3000).cuda()
+    sign = torch.where(torch.rand(3000, generator=gen) < 0.5, 1.0, -1.0)
+    p.grad = (sign * (1e-18 * (1 + torch.rand(3000, generator=gen)))).cuda()
+    opt = HipAdamW([p], lr=1e-2, eps=0.0, weight_decay=0.0, state_bits=bits)
+    opt.step()
+    want = -float(torch.tensor(1e-2)) * sign.double()
+    assert bool(((p.double().cpu() - want).abs() <= 1e-2 * (2.0 ** -150 / 1e-39 + 16 * U)).all())

@@ -343,6 +343,26 @@ def test_refusals(gpu_device):
         group_norm_act_backward(a.ref(32), x.ref(32), one, stats)
 
 
+def test_refused_workspaces_and_outputs(gpu_device):
+    from dnanet_amd.group_norm import group_norm_act, group_norm_act_backward
+    from dnanet_amd.hip import F32, HipError, PlaneBuffer
+    x = PlaneBuffer(2, 8, 5, 32, F32, "cuda", zero=True)
+    one, zero = torch.ones(32).cuda(), torch.zeros(32).cuda()
+    for ws in (torch.zeros(1 << 24), torch.zeros(1 << 24, dtype=torch.uint8), torch.zeros(1 << 24).cuda(),
+               torch.zeros(1 << 24, dtype=torch.uint8, device="cuda")[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            group_norm_act(x.ref(32), one, zero, 8, workspace=ws)
+    for plane0 in (1, 3):
+        with pytest.raises(HipError, match="overlaps"):
+            group_norm_act(x.ref(32), one, zero, 8, out=x.ref(32, plane0))
+    a, stats = group_norm_act(x.ref(32), one, zero, 8, out=x.ref(32, 4))
+    g = PlaneBuffer(2, 8, 5, 32, F32, "cuda", zero=True)
+    with pytest.raises(HipError, match="overlaps"):
+        group_norm_act_backward(g.ref(32, 4), x.ref(32, 0), one, stats, out=g.ref(32, 3))
+    with pytest.raises(HipError, match="dgamma and dbeta"):
+        group_norm_act_backward(a.ref(32, 4), x.ref(32, 0), one, stats, dgamma=one, dbeta=one)
+
+
 GIVE_UP = """
 import hashlib, sys, torch
 sys.path[:0] = [{root!r}, {tests!r}]

@@ -188,3 +188,55 @@ def test_checkpoint_round_trip(gpu_device, tmp_path):
     b.load(tmp_path)
     for p, q in zip(a.predict_batch(images), b.predict_batch(images)):
         assert (p.image == q.image).all()
+
+
+def test_capture_before_any_other_pass(gpu_device):
+    """A training step captured first of all, evaluation before its first replay: the model's group-norm workspace is zeroed when the
+    step is captured, not when it is replayed."""
+    from dnanet_amd.optim import HipAdamW
+    from dnanet_amd.unet import GraphedTrainStep
+    out = []
+    for graphed in (False, True):
+        m, x, t = make(2, 16, 5, 128, 3, 4, "silu", "bf16")
+        opt = HipAdamW(m, lr=1e-3)
+        m.train()
+        if graphed:
+            step = GraphedTrainStep(m, opt, x.cuda(), t.cuda())
+        m.eval()
+        with torch.no_grad():
+            before = m(x.cuda()).clone()
+        m.train()
+        for _ in range(3):
+            if graphed:
+                step(x.cuda(), t.cuda())
+            else:
+                m.dice_forward(m(x.cuda()), t.cuda())
+                m.backward()
+                opt.step()
+                opt.zero_grad()
+        m.eval()
+        with torch.no_grad():
+            out.append((before, m(x.cuda()).clone()))
+    assert torch.equal(out[0][0], out[1][0])
+    # the replayed step reads its learning rate in fp32: parameters differ by 2^-24 of three steps of 1e-3, logits by what that and
+    # bf16's roundings of such weights make of it: below one step of bf16 at the largest logit
+    assert float((out[0][1] - out[1][1]).abs().max()) <= 2.0 ** -7 * float(out[0][1].abs().max())
+
+
+def test_evaluation_captured_by_a_caller(gpu_device):
+    """An evaluation captured into a caller's graph keeps its results when the model has meanwhile evaluated a larger batch."""
+    m, x, _ = make(2, 16, 5, 128, 2, 4, "relu", "bf16")
+    m.eval()
+    x = x.cuda()
+    with torch.no_grad():
+        want = m(x).clone()
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            got = m(x)
+        for n in (5, 40):
+            other = m(x[:1].expand(n, -1, -1, -1).contiguous())
+            got.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want) and torch.equal(other[-1], want[0])

@@ -38,6 +38,47 @@ def test_group_norm_entry_points_refuse():
         assert backward(**kw) == 1, kw
 
 
+def test_group_norm_refuses_tensors_that_share_memory():
+    """32 channels of fp32 are 4 planes of 5 * 64 records of 32 bytes; two images of buffers of 4 (or 8) planes."""
+    from dnanet_amd import hip
+    plane, base = 5 * 64 * 32, 1 << 20
+    x, apart = hip.DnTensor(base, 4, 0, 32), hip.DnTensor(1 << 24, 4, 0, 32)
+    wide = [hip.DnTensor(base, 8, p, 32) for p in (0, 1, 3, 4)]
+
+    def forward(x, a):
+        return hip.lib.dn_group_norm_act(x, a, 2, 5, 64, 8, *[4096] * 2, 1e-5, 1, *[4096] * 5, 1 << 30, 0, None), hip.lib.dn_last_error()
+
+    for a in (hip.DnTensor(base + 32, 4, 0, 32), hip.DnTensor(base - 32, 4, 0, 32), hip.DnTensor(base + 8 * plane - 32, 4, 0, 32),
+              hip.DnTensor(base, 8, 0, 32), hip.DnTensor(base, 5, 1, 32)):
+        rc, error = forward(x, a)
+        assert rc == 1 and b"overlaps" in error, (a.base - base, error)
+    for a in wide[1:3]:
+        rc, error = forward(wide[0], a)
+        assert rc == 1 and b"overlaps" in error, (a.plane0, error)
+
+    def backward(g, x, dx, dgamma=1 << 26, dbeta=1 << 27):
+        rc = hip.lib.dn_group_norm_act_backward(g, x, dx, 2, 5, 64, 8, *[4096] * 5, 1, dgamma, dbeta, 4096, 1 << 30, 0, None)
+        return rc, hip.lib.dn_last_error()
+
+    for args, word in (((apart, x, x), b"overlaps x"), ((apart, x, hip.DnTensor(base + 4 * plane, 4, 0, 32)), b"overlaps x"),
+                       ((x, apart, hip.DnTensor(base + 32, 4, 0, 32)), b"overlaps g"), ((wide[0], apart, wide[1]), b"overlaps g"),
+                       ((x, apart, x, 4096, 4096), b"dgamma and dbeta"), ((x, apart, x, 4096, 4096 + 31 * 4), b"dgamma and dbeta")):
+        rc, error = backward(*args)
+        assert rc == 1 and word in error, (args, error)
+
+
+def test_sizes_that_no_launch_takes_are_refused():
+    """A launch holds less than 2^32 threads."""
+    from dnanet_amd import hip
+    row = (hip.DnAdamwTensor * 1)(hip.DnAdamwTensor(4096, 4096, (1 << 34) + 1, 0, 0.0, 0, 0, 0))
+    assert hip.lib.dn_adamw_step(row, 1, 4096, 4096, None, None, 32, 1e-3, 0.9, 0.999, 1e-8, 1, 0, None, 0, None) == 1
+    assert hip.lib.dn_grad_norm_workspace_bytes(row, 1) == -1
+    # one group of 2048 channels over 5 x 4096 points is more than a cluster of blocks: the form of three launches, 2^24 blocks
+    x, a = hip.DnTensor(1 << 20, 128, 0, 2048), hip.DnTensor(1 << 60, 128, 0, 2048)
+    assert hip.lib.dn_group_norm_act(x, a, 1 << 17, 5, 4096, 1, *[4096] * 2, 1e-5, 1, *[4096] * 5, 1 << 60, 1, None) == 1
+    assert b"too many" in hip.lib.dn_last_error()
+
+
 def test_adamw_entry_points_refuse():
     from dnanet_amd import hip
 
