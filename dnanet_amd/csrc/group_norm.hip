@@ -366,16 +366,14 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const unsigned
 // read.  Here a block keeps its segment in registers, publishes the segment's sums, waits for those of the other blocks of its
 // cluster -- the segments of the planes whose channels form whole groups -- and finishes from registers.
 //
-// A wait may not depend on how many blocks the chip holds or in which order it starts them: an XCD that is full of blocks which
-// wait for blocks that are to start on it would wait for ever.  Three things:
-//  * A block draws its place when it STARTS, from the counter of its shard, and consecutive places of a shard are a cluster:
-//    whatever the order, at most one cluster per shard is incomplete, and only its blocks wait for blocks to come.
-//  * There are as few shards as that the blocks of all incomplete clusters (GNF_WAITING) do not fill the slots of a single XCD,
-//    to which the blocks not yet started may all have been dealt.  (One counter alone costs 60 ns per block, one after the
-//    other: 418 us instead of 190 for 256 x 32 x 6 x 4096 bf16.  Clusters kept within an XCD: 216 us.)
-//  * A wait is bounded all the same.  A block that gives up has published its own sums; it puts its place on a list and exits,
-//    which frees its slot on the chip.  The launch's last block finds all sums published and does the listed segments over.
-// So every wait ends and every segment is written, with the same bits, whatever else runs on the GPU.
+// A cluster's blocks are consecutive in the grid.  Where each XCD starts its share of the blocks in their order, the blocks of the
+// oldest incomplete cluster are next in line everywhere and only finished clusters lie before them: nobody waits for a block that
+// waits for him.  No order is promised, though, so a wait is bounded: a block that gives up has published its own sums; it puts its
+// place on a list and exits, which frees its slot on the chip.  The launch's last block finds all sums published and does the
+// listed segments over.  So every wait ends and every segment is written, with the same bits, whatever else runs on the GPU.
+// (Places drawn from counters when a block starts need no order, but a block's loads wait for them: 182 us instead of 177 for
+// 256 x 32 x 6 x 4096 bf16, 12.7 instead of 11.9 for 2 images, and four streams of calls at once took 2.9 instead of 1.45 ms
+// a round, blocks of one launch holding the slots that another's needed.  Clusters kept within an XCD: 216 us.)
 //
 // A published word carries the launch's epoch beside its 32-bit value, so no fence and no clearing is needed: words of earlier
 // launches have other epochs.  The launch's last block counts the epoch up; counters return to zero.
@@ -385,10 +383,9 @@ constexpr int GNF_MAX_K = 64;                    // blocks of a cluster
 constexpr int GNF_MAX_CELLS = 1024;              // published cells of a cluster
 constexpr int GNF_MAX_BLOCKS = 16384;            // blocks of a launch: more images take more launches
 constexpr int GNF_POLLS = 4096;                  // looks at a word before a block gives up: about 0.6 ms
-constexpr int GNF_SHARDS = 16;                   // counters of places at most
-constexpr int GNF_WAITING = 80;                  // blocks of incomplete clusters at most: an XCD holds 96 (32 CUs x 3 blocks of 80 registers)
-constexpr int GNF_LINE = 32;                     // counters 128 bytes apart: epoch, finished shards, listed, then two per shard
-constexpr long GNF_CTRL_BYTES = (3 + 2 * GNF_SHARDS) * GNF_LINE * 4L, GNF_DEPART_BYTES = GNF_MAX_BLOCKS * 4L;
+constexpr int GNF_SHARDS = 16;                   // counters of finished clusters
+constexpr int GNF_LINE = 32;                     // counters 128 bytes apart: epoch, finished shards, listed, then the shards'
+constexpr long GNF_CTRL_BYTES = (3 + GNF_SHARDS) * GNF_LINE * 4L, GNF_DEPART_BYTES = GNF_MAX_BLOCKS * 4L;
 constexpr long GNF_LIST0 = GNF_CTRL_BYTES + GNF_DEPART_BYTES;
 constexpr long GNF_SLOT0 = GNF_LIST0 + GNF_MAX_BLOCKS * 8L;
 constexpr long GNF_END = GNF_SLOT0 + GNF_MAX_BLOCKS * 16L * 16;      // the three-launch form's partials lie behind: no word of theirs
@@ -407,9 +404,9 @@ struct GnFused {
   int m;                   // channels of a cell: gcd(channels per group, channels per record)
   int ncell;               // cells of a plane
   int ps, nsets;           // planes of a cluster, clusters of an image
-  int shards, polls;
+  int polls;
   int image0, images;      // this launch's
-  GnDiv d_most, d_shards, d_nsets, d_nseg, d_cpg, d_m;
+  GnDiv d_most, d_nsets, d_nseg, d_cpg, d_m;
   double inv_total;        // 1 / values of a group
   unsigned* ctrl;          // counters, GNF_LINE words apart
   unsigned* depart;        // per cluster: blocks that wait no longer
@@ -443,23 +440,18 @@ template <> __device__ __forceinline__ void gnf_pack4<__bf16>(uint4& v, int h, c
   if (h) { v.z = lo; v.w = hi; } else { v.x = lo; v.y = hi; }
 }
 
-struct GnPlace { int plane, seg, lo, hi, k, set, shard; long n, cluster0, cluster; unsigned place, tag; bool alone; };
+struct GnPlace { int plane, seg, lo, hi, k, set; long n, cluster0, cluster; unsigned place, tag; bool alone; };
 
 __device__ __forceinline__ unsigned gnf_count(unsigned* p) {
   return __hip_atomic_fetch_add(p, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 __device__ __forceinline__ void gnf_reset(unsigned* p) { __hip_atomic_store(p, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ int gnf_shard_clusters(const GnFused& f, int shard) {
-  return gn_div(f.d_shards, f.images * f.nsets - shard + f.shards - 1);
-}
 
-// What place `b` of shard u.shard is.  Clusters are laid out as if all had f.ps planes: plane >= P, as a cluster past the
-// last, is a block with nothing to do.
-__device__ __forceinline__ void gnf_locate(const GnFused& f, GnPlace& u, unsigned b) {
+// What block `b` is.  Clusters are laid out as if all had f.ps planes: plane >= P is a block with nothing to do (false).
+__device__ __forceinline__ bool gnf_locate(const GnFused& f, GnPlace& u, unsigned b) {
   const GnShape& s = f.s;
   u.place = b;
-  const int nth = gn_div(f.d_most, (int)b), member = (int)b - nth * (int)f.d_most.d, cluster = u.shard + f.shards * nth;
-  const int image = gn_div(f.d_nsets, cluster);
+  const int cluster = gn_div(f.d_most, (int)b), member = (int)b - cluster * (int)f.d_most.d, image = gn_div(f.d_nsets, cluster);
   u.cluster = cluster;
   u.set = cluster - image * f.nsets;
   const int plane = gn_div(f.d_nseg, member);
@@ -470,29 +462,15 @@ __device__ __forceinline__ void gnf_locate(const GnFused& f, GnPlace& u, unsigne
   u.hi = min(s.npieces, u.lo + s.seg_len);
   u.k = min(f.ps, s.P - u.set * f.ps) * s.nseg;
   u.cluster0 = u.cluster * (long)f.d_most.d;     // the cluster's first block in the slots
+  return u.plane < s.P;
 }
-// This block's place (LDS broadcast; one barrier); false: nothing to do.
-__device__ __forceinline__ bool gnf_place(const GnFused& f, unsigned* lds2, GnPlace& u) {
+// This block's place; false: nothing to do.  *missing is zeroed for after the next barrier.
+__device__ __forceinline__ bool gnf_place(const GnFused& f, unsigned* missing, GnPlace& u) {
   u.alone = f.d_most.d == 1;                           // every cluster of the launch is one block: nothing is exchanged
-  u.shard = gn_mod(f.d_shards, gn_div(f.d_most, (int)blockIdx.x));
-  if (threadIdx.x == 0) {
-    unsigned place = (unsigned)gn_div(f.d_shards, (int)blockIdx.x), epoch = 0;
-    if (!u.alone) {
-      unsigned* next = f.ctrl + (3 + 2 * u.shard) * GNF_LINE;
-      place = gnf_count(next);
-      const unsigned blocks = (unsigned)gn_div(f.d_shards, (int)gridDim.x);                         // of this shard
-      if (place == blocks - 1) gnf_reset(next);                                                     // the last to start
-      if (place >= blocks) place = blocks;                                                          // a workspace that was not zeroed
-      epoch = __hip_atomic_load(f.ctrl, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    lds2[0] = place;
-    lds2[1] = epoch;
-    lds2[2] = 0;
-  }
-  __syncthreads();
-  u.tag = (unsigned)__builtin_amdgcn_readfirstlane(lds2[1]) % 0xFFFFFFFFu + 1;         // never 0, what the workspace is filled with at first
-  gnf_locate(f, u, __builtin_amdgcn_readfirstlane(lds2[0]));                           // scalar from here on
-  return u.cluster < (long)f.images * f.nsets && u.plane < f.s.P && (u.alone || u.place < (unsigned)gn_div(f.d_shards, (int)gridDim.x));
+  if (threadIdx.x == 0) *missing = 0;
+  const unsigned epoch = u.alone ? 0 : __hip_atomic_load(f.ctrl, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  u.tag = epoch % 0xFFFFFFFFu + 1;                     // never 0, what the workspace is filled with at first
+  return gnf_locate(f, u, blockIdx.x);
 }
 
 // Sums over the wave's 32 lanes of equal record half, of four channels at a time (h: which four of the thread's half record):
@@ -562,8 +540,7 @@ __device__ __forceinline__ bool gnf_collect(const GnFused& f, const GnPlace& u, 
     if (given_up) {
       const unsigned at = gnf_count(f.ctrl + 2 * GNF_LINE);
       if (at < GNF_MAX_BLOCKS)
-        __hip_atomic_store(f.list + at, (unsigned long long)u.tag << 32 | (unsigned)u.shard << 24 | u.place, __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(f.list + at, (unsigned long long)u.tag << 32 | u.place, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");                                         // the list before the departure
     }
     *before = gnf_count(f.depart + u.cluster);
@@ -583,37 +560,36 @@ __device__ __forceinline__ void gnf_last(const GnFused& f, const GnPlace& u, uns
   *last = 0;
   if (before != (unsigned)u.k - 1) return;
   gnf_reset(f.depart + u.cluster);                                                             // the cluster's last
-  unsigned* finished = f.ctrl + (4 + 2 * u.shard) * GNF_LINE;
-  if (gnf_count(finished) != (unsigned)gnf_shard_clusters(f, u.shard) - 1) return;
+  const int shard = (int)u.cluster % GNF_SHARDS, clusters = f.images * f.nsets;
+  unsigned* finished = f.ctrl + (3 + shard) * GNF_LINE;
+  if (gnf_count(finished) != (unsigned)(clusters - shard + GNF_SHARDS - 1) / GNF_SHARDS - 1) return;
   gnf_reset(finished);                                                                         // the shard's last
-  if (gnf_count(f.ctrl + GNF_LINE) != (unsigned)min(f.shards, f.images * f.nsets) - 1) return;
+  if (gnf_count(f.ctrl + GNF_LINE) != (unsigned)min(GNF_SHARDS, clusters) - 1) return;
   gnf_reset(f.ctrl + GNF_LINE);                                                                // the launch's last
   *last = 1;
 }
 // The launch's last block: the next listed place into `u`; false: none is left, the epoch is counted up.  (One barrier.)
-__device__ __forceinline__ bool gnf_next_listed(const GnFused& f, GnPlace& u, unsigned* at, unsigned* lds2) {
+__device__ __forceinline__ bool gnf_next_listed(const GnFused& f, GnPlace& u, unsigned* at, unsigned* next) {
   __syncthreads();
   if (threadIdx.x == 0) {
-    lds2[0] = 0xFFFFFFFFu;
+    *next = 0xFFFFFFFFu;
     if (*at == 0) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
     const unsigned listed = __hip_atomic_load(f.ctrl + 2 * GNF_LINE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (*at < listed && *at < GNF_MAX_BLOCKS) {
       unsigned long long v = 0;
       for (int tries = 0; (unsigned)(v >> 32) != u.tag && tries < 1 << 22; ++tries)
         v = __hip_atomic_load(f.list + *at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      lds2[0] = (unsigned)v;
+      *next = (unsigned)v;
     } else {
       gnf_reset(f.ctrl + 2 * GNF_LINE);
       gnf_count(f.ctrl);
     }
   }
   __syncthreads();
-  const unsigned v = __builtin_amdgcn_readfirstlane(lds2[0]);
-  if (v == 0xFFFFFFFFu) return false;
+  const unsigned v = __builtin_amdgcn_readfirstlane(*next);
+  if (v >= gridDim.x) return false;                    // none (or a workspace that was not zeroed)
   ++*at;
-  u.shard = (int)(v >> 24);
-  gnf_locate(f, u, v & 0xFFFFFFu);
-  return u.cluster < (long)f.images * f.nsets && u.plane < f.s.P;
+  return gnf_locate(f, u, v);
 }
 
 __device__ __forceinline__ void gnf_wave_sum64(double& a, double& b) {
@@ -633,7 +609,7 @@ __device__ __forceinline__ int gnf_cell(const GnFused& f, const GnPlace& u, int 
 }
 
 template <int EPR> struct GnfShared {
-  unsigned place[3], last;                       // {place, epoch, missing}
+  unsigned missing, next, last;
   float red[2][GNF_WAVES * EPR], cells[GNF_MAX_CELLS * 2], gstat[EPR][2], chan[EPR][7];
 };
 
@@ -754,7 +730,7 @@ __global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_kernel(GnFused f, GnF
   constexpr int PN = Piece<T>::N, EPR = RecTraits<T>::EPR;
   __shared__ GnfShared<EPR> sh;
   GnPlace u;
-  if (!gnf_place(f, sh.place, u)) return;
+  if (!gnf_place(f, &sh.missing, u)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pc = threadIdx.x & 1, len = u.hi - u.lo;
   uint4 v[R];
   gnf_load<R>(v, o.x, o.x_pt, o.x_p0, f.s, u);
@@ -802,7 +778,7 @@ __global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_kernel(GnFused f, GnF
   unsigned before = 0;
   if (!u.alone) {
     if (owner) gnf_publish(f, u, gn_div(f.d_m, lane), cmean, m2);
-    got = gnf_collect(f, u, sh.cells, &sh.place[2], &before);
+    got = gnf_collect(f, u, sh.cells, &sh.missing, &before);
   } else {
     if (owner) { sh.cells[2 * (gn_div(f.d_m, lane))] = cmean; sh.cells[2 * (gn_div(f.d_m, lane)) + 1] = m2; }
     __syncthreads();
@@ -815,7 +791,7 @@ __global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_kernel(GnFused f, GnF
     __syncthreads();
   }
   if (u.alone || !sh.last) return;
-  for (unsigned listed = 0; gnf_next_listed(f, u, &listed, sh.place);) {       // the launch's last block: what others gave up
+  for (unsigned listed = 0; gnf_next_listed(f, u, &listed, &sh.next);) {       // the launch's last block: what others gave up
     gnf_collect_again(f, u, sh.cells);
     gnf_scales<EPR>(f, o, u, sh, [] {});
     const unsigned char* xb = (const unsigned char*)o.x + ((u.n * o.x_pt + o.x_p0 + u.plane) * (long)f.s.npieces + u.lo) * 16;
@@ -922,7 +898,7 @@ __global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_bwd_kernel(GnFused f,
   __shared__ GnfShared<EPR> sh;
   const GnShape& s = f.s;
   GnPlace u;
-  if (!gnf_place(f, sh.place, u)) return;
+  if (!gnf_place(f, &sh.missing, u)) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, pc = threadIdx.x & 1;
   uint4 vg[R], vx[R];
   gnf_load<R>(vg, o.g, o.g_pt, o.g_p0, s, u);
@@ -971,7 +947,7 @@ __global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_bwd_kernel(GnFused f,
   unsigned before = 0;
   if (!u.alone) {
     if (owner) gnf_publish(f, u, gn_div(f.d_m, lane), s1, s2);
-    got = gnf_collect(f, u, sh.cells, &sh.place[2], &before);
+    got = gnf_collect(f, u, sh.cells, &sh.missing, &before);
   } else {
     if (owner) { sh.cells[2 * (gn_div(f.d_m, lane))] = s1; sh.cells[2 * (gn_div(f.d_m, lane)) + 1] = s2; }
     __syncthreads();
@@ -984,7 +960,7 @@ __global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_bwd_kernel(GnFused f,
     __syncthreads();
   }
   if (u.alone || !sh.last) return;
-  for (unsigned listed = 0; gnf_next_listed(f, u, &listed, sh.place);) {       // the launch's last block: what others gave up
+  for (unsigned listed = 0; gnf_next_listed(f, u, &listed, &sh.next);) {       // the launch's last block: what others gave up
     gnf_channels<EPR>(f, o, u, sh);
     gnf_collect_again(f, u, sh.cells);
     gnf_scales_bwd<EPR>(f, u, sh, [] {});
@@ -1052,9 +1028,7 @@ bool gn_fused_plan(const GnShape& s, int dtype, int r, GnFused* f) {
   f->ps = std::min(s.P, s.cpg / a);              // lcm(cpg, epr) / epr planes
   f->nsets = (s.P + f->ps - 1) / f->ps;
   const long k = (long)f->ps * f->s.nseg;
-  f->shards = (int)std::max(1L, std::min<long>(GNF_SHARDS, GNF_WAITING / std::max(1L, k - 1)));
   f->d_most = gn_divisor(k);
-  f->d_shards = gn_divisor(f->shards);
   f->d_nsets = gn_divisor(f->nsets);
   f->d_nseg = gn_divisor(f->s.nseg);
   f->d_cpg = gn_divisor(s.cpg);
@@ -1081,14 +1055,13 @@ void gn_fused_workspace(GnFused* f, void* workspace) {
   f->slot = (unsigned long long*)(w + GNF_SLOT0);
 }
 bool gn_streams(const GnShape& s) { return (long)s.N * s.P * s.npieces * 16 >= GNF_STREAM_BYTES; }
-// launch(grid) for as many images at a time as a launch takes; every shard gets the same number of blocks
+// launch(grid) for as many images at a time as a launch takes
 template <typename F> void gn_fused_each(GnFused* f, F launch) {
   const long k = (long)f->ps * f->s.nseg;
   const int most = (int)std::min<long>(f->s.N, GNF_MAX_BLOCKS / (f->nsets * k));
   for (f->image0 = 0; f->image0 < f->s.N; f->image0 += most) {
     f->images = std::min(most, f->s.N - f->image0);
-    const long clusters = (long)f->images * f->nsets;
-    launch(dim3((unsigned)((clusters + f->shards - 1) / f->shards * f->shards * k)));
+    launch(dim3((unsigned)(f->images * f->nsets * k)));
   }
 }
 
