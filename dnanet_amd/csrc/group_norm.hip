@@ -372,8 +372,8 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const unsigned
 // place on a list and exits, which frees its slot on the chip.  The launch's last block finds all sums published and does the
 // listed segments over.  So every wait ends and every segment is written, with the same bits, whatever else runs on the GPU.
 // (Places drawn from counters when a block starts need no order, but a block's loads wait for them: 182 us instead of 177 for
-// 256 x 32 x 6 x 4096 bf16, 12.7 instead of 11.9 for 2 images, and four streams of calls at once took 2.9 instead of 1.45 ms
-// a round, blocks of one launch holding the slots that another's needed.  Clusters kept within an XCD: 216 us.)
+// 256 x 32 x 6 x 4096 bf16, 12.7 instead of 11.9 for 2 images, and four streams of calls at once took 2.4 to 3.1 instead
+// of 1.4 to 2.1 ms a round, blocks of one launch holding the slots that another's needed.  Clusters kept within an XCD: 216 us.)
 //
 // A published word carries the launch's epoch beside its 32-bit value, so no fence and no clearing is needed: words of earlier
 // launches have other epochs.  The launch's last block counts the epoch up; counters return to zero.
@@ -893,7 +893,7 @@ __device__ __forceinline__ void gnf_apply_bwd(const GnBackward& o, const GnShape
 }
 
 template <typename T, int ACT, int R>
-__global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_bwd_kernel(GnFused f, GnBackward o) {
+__global__ __launch_bounds__(GNF_THREADS, R <= 4 ? 6 : 4) void gn_fused_bwd_kernel(GnFused f, GnBackward o) {
   constexpr int PN = Piece<T>::N, EPR = RecTraits<T>::EPR;
   __shared__ GnfShared<EPR> sh;
   const GnShape& s = f.s;
@@ -1037,14 +1037,19 @@ bool gn_fused_plan(const GnShape& s, int dtype, int r, GnFused* f) {
   f->polls = dn_tune().gn_polls ? dn_tune().gn_polls - 1 : GNF_POLLS;
   return k <= GNF_MAX_K && k * f->ncell <= GNF_MAX_CELLS && f->nsets * k <= GNF_MAX_BLOCKS && s.C <= 1 << 15;
 }
-constexpr int GNF_R = 8, GNF_R_BWD = 4;          // 64 KB of a tensor, or 32 KB of each of two, in a block's registers
+constexpr int GNF_R = 8;                         // 64 KB of a tensor in a block's registers: three blocks on a CU
+// Backward holds 64 KB of each of two tensors: two blocks on a CU.  With 32 KB and three blocks, more of them wait for each other:
+// 301 us against 281 for 256 x 32 x 6 x 4096 bf16 (302 against 275 for 256 x 512 x 6 x 256, where 64 KB hold whole groups), 29 against 27
+// for 16 images; only up to 4 images, which leave CUs without a block, are done sooner (2: 14.0 / 15.7 us).  One size for
+// all: an image's results do not depend, not even in their last bits, on how many others are in the batch.
+constexpr int GNF_R_BWD = 8;
 // counters and published words first, at fixed places whatever the shape; the three-launch form's partials, and the partials of
 // the parameter gradients, behind them
 long gn_workspace(const GnShape& s, int dtype) {
   GnFused f;
-  const bool both = gn_fused_plan(s, dtype, GNF_R, &f) && gn_fused_plan(s, dtype, GNF_R_BWD, &f);
-  const long chunks = both ? (long)s.P * gn_param_chunks(f.s) * (dtype == DN_BF16 ? 16 : 8) * (long)sizeof(double2) : 0;
-  const long parts = std::max(gn_part_bytes(s, dtype), both ? gn_part_bytes(f.s, dtype) + chunks : 0);
+  const bool fused = gn_fused_plan(s, dtype, GNF_R_BWD, &f);
+  const long chunks = fused ? (long)s.P * gn_param_chunks(f.s) * (dtype == DN_BF16 ? 16 : 8) * (long)sizeof(double2) : 0;
+  const long parts = std::max(gn_part_bytes(s, dtype), fused ? gn_part_bytes(f.s, dtype) + chunks : 0);
   return GNF_END + parts + (long)s.N * s.G * (long)sizeof(float2) + 256;
 }
 void gn_fused_workspace(GnFused* f, void* workspace) {
@@ -1106,7 +1111,8 @@ void gn_backward_launch(dn_tensor g, dn_tensor x, dn_tensor dx, const GnShape& s
     gn_fused_each(&f, [&](dim3 grid) {
       if (rows <= 1) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, 1>), grid, dim3(GNF_THREADS), 0, st, f, o);
       else if (rows <= 2) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, 2>), grid, dim3(GNF_THREADS), 0, st, f, o);
-      else if (rows <= 3) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, 3>), grid, dim3(GNF_THREADS), 0, st, f, o);
+      else if (rows <= 4) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, 4>), grid, dim3(GNF_THREADS), 0, st, f, o);
+      else if (rows <= 6) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, 6>), grid, dim3(GNF_THREADS), 0, st, f, o);
       else hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, GNF_R_BWD>), grid, dim3(GNF_THREADS), 0, st, f, o);
     });
     const int chunks = gn_param_chunks(f.s);
