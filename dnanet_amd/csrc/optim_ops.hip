@@ -25,7 +25,8 @@ namespace {
 
 constexpr int ADAMW_MAX = 96;                 // tensors of a launch: their records fill the 4-KiB kernel argument segment
 constexpr int ADAMW_THREADS = 256;
-constexpr int ADAMW_CHUNK = 2048;             // elements of a block: a multiple of the 256-element state blocks
+constexpr int ADAMW_CHUNK = 2048;             // elements of a block, a multiple of the 256-element state blocks: all loads of a wave in
+                                              // flight at once; 4096 in two turns: 90 us instead of 88 for 27 M bf16 elements
 constexpr unsigned ADAMW_P_BF16 = 1, ADAMW_G_BF16 = 2, ADAMW_VECTOR = 4;
 
 struct AdamwEntry {                           // 40 bytes
@@ -170,6 +171,8 @@ __device__ __forceinline__ void adamw_rows32(const AdamwEntry& e, long first, in
     }
 }
 
+// Bound by HBM: 28 bytes an element with fp32 parameters and gradients, 20 with bf16.  128 M fp32 elements 672 us (5.3 TB/s, a copy's
+// rate), 12.1 M (a U-Net of four levels of 32 filters) 70 us; 46 k elements 4.2 us, a launch.
 __global__ __launch_bounds__(ADAMW_THREADS) void adamw_kernel(AdamwList list, float* exp_avg, float* exp_avg_sq, AdamwArgs a) {
   const AdamwEntry e = list.e[adamw_find(list, blockIdx.x)];
   const AdamwScalars s = adamw_scalars(a);
@@ -312,6 +315,8 @@ __device__ __forceinline__ void adamw_rows8(const AdamwEntry& e, long first, int
     }
 }
 
+// 16 bytes an element with fp32 parameters and gradients: bound by HBM, 128 M elements 373 us (5.5 TB/s), 12.1 M 41 us.  With bf16, 10
+// bytes: 284 us (4.5 TB/s), the vector units are busy for most of it (90 instructions an element, 16 of them fp64).
 __global__ __launch_bounds__(ADAMW_THREADS) void adamw8_kernel(AdamwList list, unsigned char* exp_avg, unsigned char* exp_avg_sq,
                                                                float* m_scale, float* v_scale, AdamwArgs a) {
   const AdamwEntry e = list.e[adamw_find(list, blockIdx.x)];
@@ -365,7 +370,8 @@ __global__ void adamw_hyper_kernel(float* hyper, long long* step, double beta1, 
   }
 }
 
-// ---- global gradient norm: squares in fp64 (no overflow, no order that matters beyond 2^-53), fixed order ------------------
+// ---- global gradient norm: squares in fp64 (no overflow, no order that matters beyond 2^-53), fixed order.  One read of the gradients,
+// which the step then finds in the last-level cache if they fit there (256 MB): 8 us more for a step over 12.1 M elements, of 70.
 template <int WAVES> __device__ __forceinline__ double adamw_block_sum(double v) {
   __shared__ double red[WAVES];
 #pragma unroll

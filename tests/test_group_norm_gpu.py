@@ -117,6 +117,17 @@ def test_backward(gpu_device, shape, dtype, act):
     assert torch.equal(gbuf.data, dx.data)
 
 
+# groups (or planes) of 96, 120 and 192 blocks, and of 384, which take the form of three launches
+LARGE = [(2, 128, 1, 6, 4096), (1, 40, 4, 6, 40000), (1, 16, 2, 6, 65536), (1, 512, 1, 6, 4096)]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", LARGE)
+def test_large_groups(gpu_device, shape, dtype):
+    test_forward(gpu_device, shape, dtype, "silu")
+    test_backward(gpu_device, shape, dtype, "relu")
+
+
 def test_backward_agrees_with_differences(gpu_device):
     """L = sum(w * a): <dx, d> + <dgamma, dg> + <dbeta, db> of the kernels against the change of the definition's L along that
     direction, in 64 bits: the quotient's own error is step^2 / 6 of a third derivative (below 4 sum|w|), the kernels' 64 u of
