@@ -316,7 +316,7 @@ __device__ __forceinline__ void adamw_rows8(const AdamwEntry& e, long first, int
 }
 
 // 16 bytes an element with fp32 parameters and gradients: bound by HBM, 128 M elements 373 us (5.5 TB/s), 12.1 M 41 us.  With bf16, 10
-// bytes: 284 us (4.5 TB/s), the vector units are busy for most of it (90 instructions an element, 16 of them fp64).
+// bytes: 284 us (4.5 TB/s), the vector units are busy for most of it (61 instructions an element, 10 of them fp64 or conversions to it).
 __global__ __launch_bounds__(ADAMW_THREADS) void adamw8_kernel(AdamwList list, unsigned char* exp_avg, unsigned char* exp_avg_sq,
                                                                float* m_scale, float* v_scale, AdamwArgs a) {
   const AdamwEntry e = list.e[adamw_find(list, blockIdx.x)];
