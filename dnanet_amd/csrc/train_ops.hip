@@ -177,7 +177,12 @@ __device__ __forceinline__ void bn_finalize_channel(int c, double s, double ss, 
   shift[c] = beta[c] - (float)mean * sc;
   if (running_mean) {
     const double unbiased = count > 1 ? var * count / (count - 1) : var;
-    running_mean[c] = (1.f - momentum) * running_mean[c] + momentum * (float)mean;
+    {
+#pragma clang fp contract(off)      // products and sum rounded separately, whatever instructions the build may use
+      const float keep = (1.f - momentum) * running_mean[c];
+      const float take = momentum * (float)mean;
+      running_mean[c] = keep + take;
+    }
     running_var[c] = (1.f - momentum) * running_var[c] + momentum * (float)unbiased;
   }
 }
