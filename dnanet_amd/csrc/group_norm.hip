@@ -93,6 +93,21 @@ __device__ __forceinline__ GnUnit gn_unit(const GnShape& s) {
   return u;
 }
 
+// Slots past the last channel of a partial plane come out as zero, whatever they hold (0 * NaN would be NaN): the bits of this
+// thread's half records that are kept.  Sums need no mask: those of unused slots are their own, and nobody reads them.
+template <typename T> __device__ __forceinline__ uint4 gn_kept_bits(const GnShape& s, int plane) {
+  constexpr int PN = Piece<T>::N;
+  const int left = s.C - plane * RecTraits<T>::EPR - (int)(threadIdx.x & 1) * PN;
+  unsigned b[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (PN == 4) b[j] = left > j ? ~0u : 0u;
+    else b[j] = (left > 2 * j ? 0xFFFFu : 0u) | (left > 2 * j + 1 ? 0xFFFF0000u : 0u);
+  }
+  return make_uint4(b[0], b[1], b[2], b[3]);
+}
+__device__ __forceinline__ uint4 gn_and(const uint4& v, const uint4& m) { return make_uint4(v.x & m.x, v.y & m.y, v.z & m.z, v.w & m.w); }
+
 // part[cell][channel of the plane] = (mean, M2) of the segment
 template <typename T>
 __global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(const unsigned char* x, int pt, int p0, GnShape s, float2* part) {
@@ -175,9 +190,10 @@ __global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(const unsigned cha
   float sc[PN], sh[PN];
 #pragma unroll
   for (int j = 0; j < PN; ++j) { sc[j] = scale[c0 + j]; sh[j] = shift[c0 + j]; }
+  const uint4 kept = gn_kept_bits<T>(s, u.plane);
   for (int i = u.lo + threadIdx.x; i < u.hi; i += GN_THREADS) {
     float f[PN];
-    Piece<T>::unpack(*(const uint4*)(xb + (long)i * 16), f);
+    Piece<T>::unpack(gn_and(*(const uint4*)(xb + (long)i * 16), kept), f);
 #pragma unroll
     for (int j = 0; j < PN; ++j) f[j] = gn_act<ACT>(fmaf(f[j], sc[j], sh[j]));
     *(uint4*)(ab + (long)i * 16) = Piece<T>::pack(f);
@@ -346,10 +362,11 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const unsigned
     c1[j] = cf.x;
     c2[j] = cf.y;
   }
+  const uint4 kept = gn_kept_bits<T>(s, u.plane);
   for (int i = u.lo + threadIdx.x; i < u.hi; i += GN_THREADS) {
     float fg[PN], fx[PN];
-    Piece<T>::unpack(*(const uint4*)(gb + (long)i * 16), fg);
-    Piece<T>::unpack(*(const uint4*)(xb + (long)i * 16), fx);
+    Piece<T>::unpack(gn_and(*(const uint4*)(gb + (long)i * 16), kept), fg);
+    Piece<T>::unpack(gn_and(*(const uint4*)(xb + (long)i * 16), kept), fx);
 #pragma unroll
     for (int j = 0; j < PN; ++j) {
       const float dz = gn_act_grad<ACT>(fmaf(fx[j], k.sc[j], k.sh[j]), fg[j]);
@@ -706,8 +723,9 @@ __device__ __forceinline__ void gnf_scales(const GnFused& f, const GnForward& o,
   leave();
   __syncthreads();
 }
-// Pieces first, first + GNF_THREADS, ... of the segment: v = act(v * scale + shift), stored.
-template <typename T, int ACT, int R>
+// Pieces first, first + GNF_THREADS, ... of the segment: v = act(v * scale + shift), stored.  PARTIAL: channels do not fill the last plane's
+// records (an instance of its own: where all instances looked for such planes, a branch that no block took cost 12 us of 276).
+template <typename T, int ACT, int R, bool PARTIAL>
 __device__ __forceinline__ void gnf_apply(const GnForward& o, const GnShape& s, const GnPlace& u, uint4 (&v)[R], int first,
                                           const GnfShared<RecTraits<T>::EPR>& sh) {
   constexpr int PN = Piece<T>::N;
@@ -726,13 +744,13 @@ __device__ __forceinline__ void gnf_apply(const GnForward& o, const GnShape& s, 
       for (int j = 0; j < 4; ++j) t[j] = gn_act<ACT>(fmaf(t[j], sc[j], sf[j]));
       gnf_pack4<T>(v[k], h, t);
       const int i = first + k * GNF_THREADS;
-      if (h == PN / 4 - 1 && i < len) gnf_store(ab + (unsigned)i * 16u, v[k], o.stream);
+      if (h == PN / 4 - 1 && i < len) gnf_store(ab + (unsigned)i * 16u, PARTIAL ? gn_and(v[k], gn_kept_bits<T>(s, u.plane)) : v[k], o.stream);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
 
-template <typename T, int ACT, int R>
+template <typename T, int ACT, int R, bool PARTIAL = false>
 __global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_kernel(GnFused f, GnForward o) {
   constexpr int PN = Piece<T>::N, EPR = RecTraits<T>::EPR;
   __shared__ GnfShared<EPR> sh;
@@ -792,7 +810,7 @@ __global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_kernel(GnFused f, GnF
   }
   if (got) {
     gnf_scales<EPR>(f, o, u, sh, [&] { gnf_last(f, u, before, &sh.last); });
-    gnf_apply<T, ACT, R>(o, f.s, u, v, threadIdx.x, sh);
+    gnf_apply<T, ACT, R, PARTIAL>(o, f.s, u, v, threadIdx.x, sh);
   } else {
     gnf_last(f, u, before, &sh.last);
     __syncthreads();
@@ -805,7 +823,7 @@ __global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_kernel(GnFused f, GnF
 #pragma unroll 1
     for (int i = threadIdx.x; i < u.hi - u.lo; i += GNF_THREADS) {
       uint4 one[1] = {*(const uint4*)(xb + (unsigned)i * 16u)};
-      gnf_apply<T, ACT, 1>(o, f.s, u, one, i, sh);
+      gnf_apply<T, ACT, 1, PARTIAL>(o, f.s, u, one, i, sh);
     }
   }
 }
@@ -866,7 +884,7 @@ __device__ __forceinline__ void gnf_scales_bwd(const GnFused& f, const GnPlace& 
   __syncthreads();
 }
 // Pieces first, first + GNF_THREADS, ... of the segment: dx, stored.  MASKED: vg holds dz already (ReLU).
-template <typename T, int ACT, int R, bool MASKED>
+template <typename T, int ACT, int R, bool MASKED, bool PARTIAL>
 __device__ __forceinline__ void gnf_apply_bwd(const GnBackward& o, const GnShape& s, const GnPlace& u, uint4 (&vg)[R], uint4 (&vx)[R],
                                               int first, const GnfShared<RecTraits<T>::EPR>& sh) {
   constexpr int PN = Piece<T>::N;
@@ -893,13 +911,13 @@ __device__ __forceinline__ void gnf_apply_bwd(const GnBackward& o, const GnShape
       }
       gnf_pack4<T>(vg[k], h, fg);
       const int i = first + k * GNF_THREADS;
-      if (h == PN / 4 - 1 && i < len) gnf_store(db + (unsigned)i * 16u, vg[k], o.stream);
+      if (h == PN / 4 - 1 && i < len) gnf_store(db + (unsigned)i * 16u, PARTIAL ? gn_and(vg[k], gn_kept_bits<T>(s, u.plane)) : vg[k], o.stream);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
 }
 
-template <typename T, int ACT, int R>
+template <typename T, int ACT, int R, bool PARTIAL = false>
 __global__ __launch_bounds__(GNF_THREADS, R <= 4 ? 6 : 4) void gn_fused_bwd_kernel(GnFused f, GnBackward o) {
   constexpr int PN = Piece<T>::N, EPR = RecTraits<T>::EPR;
   __shared__ GnfShared<EPR> sh;
@@ -961,7 +979,7 @@ __global__ __launch_bounds__(GNF_THREADS, R <= 4 ? 6 : 4) void gn_fused_bwd_kern
   }
   if (got) {
     gnf_scales_bwd<EPR>(f, u, sh, [&] { gnf_last(f, u, before, &sh.last); });
-    gnf_apply_bwd<T, ACT, R, true>(o, s, u, vg, vx, threadIdx.x, sh);
+    gnf_apply_bwd<T, ACT, R, true, PARTIAL>(o, s, u, vg, vx, threadIdx.x, sh);
   } else {
     gnf_last(f, u, before, &sh.last);
     __syncthreads();
@@ -976,7 +994,7 @@ __global__ __launch_bounds__(GNF_THREADS, R <= 4 ? 6 : 4) void gn_fused_bwd_kern
 #pragma unroll 1
     for (int i = threadIdx.x; i < u.hi - u.lo; i += GNF_THREADS) {
       uint4 one_g[1] = {*(const uint4*)(gb + (unsigned)i * 16u)}, one_x[1] = {*(const uint4*)(xb + (unsigned)i * 16u)};
-      gnf_apply_bwd<T, ACT, 1, false>(o, s, u, one_g, one_x, i, sh);
+      gnf_apply_bwd<T, ACT, 1, false, PARTIAL>(o, s, u, one_g, one_x, i, sh);
     }
   }
 }
@@ -1088,7 +1106,8 @@ void gn_forward_launch(dn_tensor x, dn_tensor a, const GnShape& s, const float* 
                       gn_streams(s)};
     const int rows = (f.s.seg_len + GNF_THREADS - 1) / GNF_THREADS;            // pieces of a thread
     gn_fused_each(&f, [&](dim3 grid) {
-      if (rows <= 2) hipLaunchKernelGGL((gn_fused_kernel<T, ACT, 2>), grid, dim3(GNF_THREADS), 0, st, f, o);
+      if (s.C % EPR) hipLaunchKernelGGL((gn_fused_kernel<T, ACT, GNF_R, true>), grid, dim3(GNF_THREADS), 0, st, f, o);
+      else if (rows <= 2) hipLaunchKernelGGL((gn_fused_kernel<T, ACT, 2>), grid, dim3(GNF_THREADS), 0, st, f, o);
       else if (rows <= 4) hipLaunchKernelGGL((gn_fused_kernel<T, ACT, 4>), grid, dim3(GNF_THREADS), 0, st, f, o);
       else if (rows <= 6) hipLaunchKernelGGL((gn_fused_kernel<T, ACT, 6>), grid, dim3(GNF_THREADS), 0, st, f, o);
       else hipLaunchKernelGGL((gn_fused_kernel<T, ACT, GNF_R>), grid, dim3(GNF_THREADS), 0, st, f, o);
@@ -1116,7 +1135,8 @@ void gn_backward_launch(dn_tensor g, dn_tensor x, dn_tensor dx, const GnShape& s
                        gamma, mean, rstd, scale, shift, part, gn_streams(s)};
     const int rows = (f.s.seg_len + GNF_THREADS - 1) / GNF_THREADS;
     gn_fused_each(&f, [&](dim3 grid) {
-      if (rows <= 1) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, 1>), grid, dim3(GNF_THREADS), 0, st, f, o);
+      if (s.C % EPR) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, GNF_R_BWD, true>), grid, dim3(GNF_THREADS), 0, st, f, o);
+      else if (rows <= 1) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, 1>), grid, dim3(GNF_THREADS), 0, st, f, o);
       else if (rows <= 2) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, 2>), grid, dim3(GNF_THREADS), 0, st, f, o);
       else if (rows <= 4) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, 4>), grid, dim3(GNF_THREADS), 0, st, f, o);
       else if (rows <= 6) hipLaunchKernelGGL((gn_fused_bwd_kernel<T, ACT, 6>), grid, dim3(GNF_THREADS), 0, st, f, o);

@@ -183,6 +183,33 @@ def test_non_finite_values_stay_in_their_group(gpu_device, value, act):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 12, 3, 5, 300), (3, 20, 5, 2, 4096), (2, 36, 9, 6, 40), (1, 515, 1, 2, 4096)])
+def test_slots_past_the_channels_may_hold_anything(gpu_device, shape, dtype):
+    """NaN and infinities in a partial plane's unused slots: the results of zeros there, zeros in those slots of the outputs."""
+    from dnanet_amd import hip
+    from dnanet_amd.group_norm import group_norm_act, group_norm_act_backward
+    from dnanet_amd.hip import PlaneBuffer
+    n, c, groups, h, w = shape
+    clean, _, gamma, beta = make(shape, dtype, seed=4)
+    gamma, beta, epr = gamma.cuda(), beta.cuda(), hip.epr(clean.dtype)
+    grad = PlaneBuffer.wrap(clean.data.flip(-2).contiguous())
+    dirty = [PlaneBuffer.wrap(b.data.clone()) for b in (clean, grad)]
+    used = c % epr
+    assert used
+    for b, value in zip(dirty, (float("nan"), float("inf"))):
+        b.data[:, -1, :, :, used:] = value
+        b.data[:, -1, ::2, :, used:] = -value
+    results = []
+    for x, g in ((clean, grad), dirty):
+        a, stats = group_norm_act(x.ref(c), gamma, beta, groups, EPS, "silu")
+        dx, dgamma, dbeta = group_norm_act_backward(g.ref(c), x.ref(c), gamma, stats)
+        results.append((a.data, dx.data, stats.mean, stats.rstd, stats.scale, stats.shift, dgamma, dbeta))
+    for want, got in zip(*results):
+        assert torch.equal(got, want)
+    assert not results[1][0][:, -1, :, :, used:].any() and not results[1][1][:, -1, :, :, used:].any()
+
+
 def test_constant_group(gpu_device):
     """Variance 0: rstd = eps^-1/2 = 316, z = beta up to one rounding of the shift (3 * 316), and the gradient is finite."""
     from dnanet_amd.group_norm import group_norm_act, group_norm_act_backward
