@@ -20,6 +20,9 @@ ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}      # DN_ACT_*
 
 
 def parse_activation(activation: str) -> int:
+    code = ACTIVATIONS.get(activation)
+    if code is not None:
+        return code
     try:
         return ACTIVATIONS[str(activation).lower()]
     except KeyError:
@@ -53,14 +56,19 @@ class GroupNormStats:
         if self._parts is not None:
             return self._parts[k]
         n, groups, pad = self._shape
+        flat = self.flat
         if k < 2:
-            return self.flat.as_strided((n, groups), (groups, 1), self.flat.storage_offset() + k * n * groups)
-        return self.flat.as_strided((n, pad), (pad, 1), self.flat.storage_offset() + n * (2 * groups + (k - 2) * pad))
+            return flat.as_strided((n, groups), (groups, 1), flat.storage_offset() + k * n * groups)
+        return flat.as_strided((n, pad), (pad, 1), flat.storage_offset() + n * (2 * groups + (k - 2) * pad))
 
     mean = property(lambda self: self._part(0))
     rstd = property(lambda self: self._part(1))
     scale = property(lambda self: self._part(2))
     shift = property(lambda self: self._part(3))
+
+    def _spread(self, base: int) -> Tuple[int, int, int, int]:
+        n, groups, pad = self._shape
+        return base, base + 4 * n * groups, base + 8 * n * groups, base + 8 * n * groups + 4 * n * pad
 
     def _pointers(self, n: int, channels: int, groups: int, device: torch.device) -> Tuple[int, int, int, int]:
         """Device pointers of the four, checked against a call's sizes."""
@@ -68,8 +76,7 @@ class GroupNormStats:
         if self._parts is None:
             if self._shape != (n, groups, pad):
                 raise ValueError(f"stats.mean is of {self._shape[0]} images and {self._shape[1]} groups, the call of {n} and {groups}")
-            base = _vector(self.flat, (2 * n * (groups + pad),), device, "stats.flat")
-            return base, base + 4 * n * groups, base + 8 * n * groups, base + 8 * n * groups + 4 * n * pad
+            return self._spread(_vector(self.flat, (2 * n * (groups + pad),), device, "stats.flat"))
         mean, rstd, scale, shift = self._parts
         return (_vector(mean, (n, groups), device, "stats.mean"), _vector(rstd, (n, groups), device, "stats.rstd"),
                 _vector(scale, (n, pad), device, "stats.scale"), _vector(shift, (n, pad), device, "stats.shift"))
@@ -113,6 +120,14 @@ def _same(buf: PlaneBuffer, like: PlaneBuffer, what: str):
                          f"{like.data.dtype} on {like.data.device}")
 
 
+def _like(src: PlaneBuffer, channels: int) -> PlaneBuffer:
+    """A new buffer of ``channels`` channels and the sizes of ``src``."""
+    buf = PlaneBuffer.__new__(PlaneBuffer)
+    buf.n, buf.planes_total, buf.h, buf.w, buf.dtype = src.n, hip.planes(channels, src.dtype), src.h, src.w, src.dtype
+    buf.data = src.data.new_empty((buf.n, buf.planes_total, buf.h, buf.w, src.data.shape[4]))
+    return buf
+
+
 def _vector(t: torch.Tensor, shape, device, what: str) -> int:
     if t.dtype != torch.float32 or t.shape != shape or t.device != device or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous float32 tensor of shape {tuple(shape)} on {device}, got {tuple(t.shape)} {t.dtype} "
@@ -141,24 +156,26 @@ def group_norm_act(x: DnTensor, gamma: torch.Tensor, beta: torch.Tensor, groups:
     the statistics go (default: new tensors); ``workspace``: a caller's own (uint8, zeroed before its first use, one call at
     a time).  Returns the output's buffer and the statistics for the backward call."""
     src = _owner(x, "x")
-    act, c, dev = parse_activation(activation), x.channels, src.data.device
-    need = _need(src.n, c, src.h, src.w, groups, src.dtype)
-    g, b = _vector(gamma, (c,), dev, "gamma"), _vector(beta, (c,), dev, "beta")
+    act, c, data = parse_activation(activation), x.channels, src.data
+    n, h, w, dtype, dev = src.n, src.h, src.w, src.dtype, data.device
+    need = _need(n, c, h, w, groups, dtype)
+    shape = (c,)
+    g, b = _vector(gamma, shape, dev, "gamma"), _vector(beta, shape, dev, "beta")
     if out is None:
-        dst = PlaneBuffer(src.n, hip.planes(c, src.dtype), src.h, src.w, src.dtype, dev)
+        dst = _like(src, c)
         out = dst.ref(c)
     else:
         dst = _owner(out, "out")
         _same(dst, src, "out")
     if stats is None:
-        flat = torch.empty(GroupNormStats.floats(src.n, c, groups), dtype=torch.float32, device=dev)
-        stats = GroupNormStats.from_flat(flat, src.n, c, groups, activation)
-    vectors = stats._pointers(src.n, c, groups, dev)
+        stats = GroupNormStats.from_flat(gamma.new_empty(GroupNormStats.floats(n, c, groups)), n, c, groups, activation)
+        vectors = stats._spread(stats.flat.data_ptr())
+    else:
+        vectors = stats._pointers(n, c, groups, dev)
     with _on(dev):
         stream = hip.raw_stream(dev)
         ws = _workspace(dev, stream, need) if workspace is None else _given_workspace(workspace, dev)
-        hip.check(hip.lib.dn_group_norm_act(x, out, src.n, src.h, src.w, groups, g, b, eps, act, *vectors, ws.data_ptr(), ws.numel(),
-                                            src.dtype, stream))
+        hip.check(hip.lib.dn_group_norm_act(x, out, n, h, w, groups, g, b, eps, act, *vectors, ws.data_ptr(), ws.numel(), dtype, stream))
     stats.groups, stats.activation = groups, activation
     return dst, stats
 
@@ -174,19 +191,24 @@ def group_norm_act_backward(g: DnTensor, x: DnTensor, gamma: torch.Tensor, stats
     need = _need(src.n, c, src.h, src.w, groups, src.dtype)
     ga = _vector(gamma, (c,), dev, "gamma")
     if out is None:
-        dst = PlaneBuffer(src.n, hip.planes(c, src.dtype), src.h, src.w, src.dtype, dev)
+        dst = _like(src, c)
         out = dst.ref(c)
     else:
         dst = _owner(out, "out")
         _same(dst, src, "out")
         if dst.data.data_ptr() == src.data.data_ptr() and abs(out.plane0 - x.plane0) < hip.planes(c, src.dtype):
             raise ValueError("out must not overlap x")
-    if dgamma is None:
-        dgamma = torch.empty(c, dtype=torch.float32, device=dev)
-    if dbeta is None:
-        dbeta = torch.empty(c, dtype=torch.float32, device=dev)
     vectors = stats._pointers(src.n, c, groups, dev)
-    dg, db = _vector(dgamma, (c,), dev, "dgamma"), _vector(dbeta, (c,), dev, "dbeta")
+    if dgamma is None:
+        dgamma = gamma.new_empty(c)
+        dg = dgamma.data_ptr()
+    else:
+        dg = _vector(dgamma, (c,), dev, "dgamma")
+    if dbeta is None:
+        dbeta = gamma.new_empty(c)
+        db = dbeta.data_ptr()
+    else:
+        db = _vector(dbeta, (c,), dev, "dbeta")
     with _on(dev):
         stream = hip.raw_stream(dev)
         ws = _workspace(dev, stream, need) if workspace is None else _given_workspace(workspace, dev)

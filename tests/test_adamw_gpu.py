@@ -433,3 +433,41 @@ def test_denormal_second_moments_without_eps(gpu_device, bits):
     opt.step()
     want = -float(torch.tensor(1e-2)) * sign.double()
     assert bool(((p.double().cpu() - want).abs() <= 1e-2 * (2.0 ** -150 / 1e-39 + 16 * U)).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_unaligned_bf16_with_clipping(gpu_device, bits):
+    """bf16 parameters and gradients that start at an odd element: as the same values in tensors of their own."""
+    from dnanet_amd.optim import HipAdamW
+    out = []
+    for shift in (0, 1):
+        gen = torch.Generator().manual_seed(8)
+        params = []
+        for n in (1, 5, 300, 5000):
+            p = torch.zeros(n + shift, dtype=torch.bfloat16).cuda()[shift:]
+            g = torch.zeros(n + shift, dtype=torch.bfloat16).cuda()[shift:]
+            p.copy_(torch.randn(n, generator=gen))
+            g.copy_(torch.randn(n, generator=gen))
+            p.grad = g
+            params.append(p)
+        opt = HipAdamW(params, lr=1e-2, state_bits=bits, max_grad_norm=0.5)
+        for _ in range(3):
+            opt.step()
+        # the norm's partial sums are the same numbers added in another order: fp64, then one rounding to fp32 of norm and coefficient
+        out.append((float(opt.grad_norm), torch.cat(params).float().cpu()))
+    assert abs(out[0][0] - out[1][0]) <= 2 * U * out[0][0]
+    # three steps of 1e-2 from gradients that differ by 2^-23: a parameter rounds to the same bf16 value or to its neighbour
+    assert bool(((out[0][1] - out[1][1]).abs() <= 3 * 2.0 ** -8 * out[0][1].abs() + 3e-2 * 2.0 ** -8).all())
+
+
+def test_a_parameter_that_changes_its_size_is_refused(gpu_device):
+    from dnanet_amd.optim import HipAdamW
+    p = torch.randn(300).cuda()
+    p.grad = torch.randn(300).cuda()
+    opt = HipAdamW([p])
+    opt.step()
+    p.grad = None
+    p.data = torch.randn(70000).cuda()
+    p.grad = torch.randn(70000).cuda()
+    with pytest.raises(ValueError, match="new optimizer"):
+        opt.step()
