@@ -128,6 +128,14 @@ def test_large_groups(gpu_device, shape, dtype):
     test_backward(gpu_device, shape, dtype, "relu")
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("shape", [(600, 24, 3, 1, 9), (140, 64, 8, 2, 300), (129, 64, 4, 1, 65), (127, 64, 4, 1, 65)])
+def test_many_images(gpu_device, shape, dtype):
+    """Around and past the number of blocks up to which a launch sums the parameter gradients itself."""
+    test_forward(gpu_device, shape, dtype, "relu")
+    test_backward(gpu_device, shape, dtype, "silu")
+
+
 def test_backward_agrees_with_differences(gpu_device):
     """L = sum(w * a): <dx, d> + <dgamma, dg> + <dbeta, db> of the kernels against the change of the definition's L along that
     direction, in 64 bits: the quotient's own error is step^2 / 6 of a third derivative (below 4 sum|w|), the kernels' 64 u of
