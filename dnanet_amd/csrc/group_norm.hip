@@ -935,7 +935,10 @@ __device__ __forceinline__ void gnf_scales_bwd(const GnFused& f, const GnPlace& 
   leave();
   __syncthreads();
 }
-// Pieces first, first + GNF_THREADS, ... of the segment: dx, stored.  MASKED: vg holds dz already (ReLU).
+// Whether dz can take the place of g in the registers between the passes, without another rounding: ReLU's is g or 0, fp32 holds any.
+// (SiLU's in bf16 is computed twice.)
+template <typename T, int ACT> constexpr bool gnf_keeps_dz() { return ACT == DN_ACT_RELU || sizeof(T) == 4; }
+// Pieces first, first + GNF_THREADS, ... of the segment: dx, stored.  MASKED: vg holds dz already where it can.
 template <typename T, int ACT, int R, bool MASKED, bool PARTIAL>
 __device__ __forceinline__ void gnf_apply_bwd(const GnBackward& o, const GnShape& s, const GnPlace& u, uint4 (&vg)[R], uint4 (&vx)[R],
                                               int first, const GnfShared<RecTraits<T>::EPR>& sh) {
@@ -958,7 +961,7 @@ __device__ __forceinline__ void gnf_apply_bwd(const GnBackward& o, const GnShape
       gnf_unpack4<T>(vx[k], h, fx);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float dz = ACT == DN_ACT_SILU || !MASKED ? gn_act_grad<ACT>(fmaf(fx[j], sc[j], sf[j]), fg[j]) : fg[j];
+        const float dz = MASKED && gnf_keeps_dz<T, ACT>() ? fg[j] : gn_act_grad<ACT>(fmaf(fx[j], sc[j], sf[j]), fg[j]);
         fg[j] = fmaf(k4[j], dz, fmaf(k6[j], fx[j] - mu[j], k5[j]));
       }
       gnf_pack4<T>(vg[k], h, fg);
@@ -1003,7 +1006,7 @@ __global__ __launch_bounds__(GNF_THREADS, R <= 4 ? 6 : 4) void gn_fused_bwd_kern
         fg[j] = dz;
         asm volatile("" : "+v"(a1[j]), "+v"(a2[j]));                           // both here: one put off would keep dz and x alive
       }
-      if constexpr (ACT == DN_ACT_RELU) gnf_pack4<T>(vg[k], h, fg);            // g or 0: dz fits where g was
+      if constexpr (gnf_keeps_dz<T, ACT>()) gnf_pack4<T>(vg[k], h, fg);
       __builtin_amdgcn_sched_barrier(0);
     }
     gnf_wave_sums<PN>(a1, h, sh.red[0]);
