@@ -6,7 +6,7 @@ A plane-record tensor is ``[N][planes][H][W][record]``: 16 bf16 or 8 fp32 channe
 
 The 8-bit states are e4m3 codes with one fp32 scale per 256 consecutive elements of a tensor (value = code * scale).  The
 scale is the smallest power of two that brings the block's largest magnitude to 448 or below; a magnitude is rounded up or
-down at random in proportion (16 bits of a hash of the element's place in the moment buffers, step and seed), a second moment above zero keeps at least the
+down at random in proportion (16 bits of a hash of element, step and seed), a second moment above zero keeps at least the
 smallest code.
 """
 import math
@@ -210,10 +210,13 @@ def prepare(case, seed):
 def _own_optimizer(s):
     from dnanet_amd.optim import HipAdamW
     case = s["case"]
-    params, grads = ([s[name][at:at + n] for n, at in zip(s["sizes"], s["starts"])] for name in ("p", "g"))
+    params = []
+    for n, at in zip(s["sizes"], s["starts"]):
+        p = s["p"][at:at + n]
+        p.grad = s["g"][at:at + n]
+        params.append(p)
     weights = sum(1 for d in s["decay"] if d)
-    groups = [{"params": params[:weights], "grads": grads[:weights], "weight_decay": DECAY},
-              {"params": params[weights:], "grads": grads[weights:], "weight_decay": 0.0}]
+    groups = [{"params": params[:weights], "weight_decay": DECAY}, {"params": params[weights:], "weight_decay": 0.0}]
     opt = HipAdamW([group for group in groups if group["params"]], lr=LR, betas=(BETA1, BETA2), eps=ADAM_EPS,
                    state_bits=case["bits"], max_grad_norm=case["clip"] or None, seed=s["seed"])
     opt.step_count = FIRST_STEP
@@ -350,7 +353,11 @@ def _plain_adamw(s):
         m = BETA1 * old_m + (1.0 - BETA1) * gd
         v = BETA2 * old_v + (1.0 - BETA2) * gd * gd
         del old_m, old_v, gd
-        bits = _hash(torch.arange(s["total"], device=p.device), t, s["seed"]).view(-1, BLOCK)
+        index = torch.arange(s["total"], device=p.device)
+        index = index - torch.repeat_interleave(torch.tensor(s["starts"], device=p.device), s["lengths"], output_size=s["total"])
+        number = torch.repeat_interleave(torch.arange(len(s["sizes"]), device=p.device), s["lengths"], output_size=s["total"])
+        bits = _hash((index + number * 0xC2B2AE35) & 0xFFFFFFFF, t, s["seed"]).view(-1, BLOCK)
+        del index, number
         for name, x, b in (("m", m, bits & 0xFFFF), ("v", v, bits >> 16)):
             y = x.abs().float()
             fraction, exponent = torch.frexp(y.amax(1))            # fraction in [0.5, 1); 448 = 0.875 * 2 ** 9
@@ -437,7 +444,7 @@ def _exact_adamw(s):
                 old = old * s[name + "_scale"][at // BLOCK:at // BLOCK + (n + BLOCK - 1) // BLOCK].double().repeat_interleave(BLOCK)[:n]
             moments[name] = old * beta + x * (1.0 - beta)
         if eight:
-            key = torch.arange(at, at + n, device=g.device) + t * 0x9E3779B9 + s["seed"] * 0x85EBCA6B
+            key = torch.arange(n, device=g.device) + (k * 0xC2B2AE35 & 0xFFFFFFFF) + t * 0x9E3779B9 + s["seed"] * 0x85EBCA6B
             for shift, factor in ((16, 0x7FEB352D), (15, 0x846CA68B)):
                 key = key % (1 << 32)
                 key = (key ^ (key >> shift)) * factor
