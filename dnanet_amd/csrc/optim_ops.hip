@@ -11,8 +11,8 @@
 // 8-bit moments: e4m3 codes and one fp32 scale per 256 consecutive elements of a tensor, the smallest power of two that brings
 // the block's largest magnitude to 448 or below (a power of two: dividing by it rounds nothing, so a code depends on the new
 // moment alone).  Rounding is stochastic, up with the probability of the remainder, 16 bits of a hash of
-// (place in the moment buffers, step, seed) for each moment: to nearest, a second moment would stand still as soon as one step moves it by less than half a code step
-// (2^-4 of its value, where 1 - beta2 is 2^-10).  A second moment above zero keeps at least the smallest code: m / (0 + eps)
+// (tensor's number, element in the tensor, step, seed) for each moment: to nearest, a second moment would stand still as soon as
+// one step moves it by less than half a code step (2^-4 of its value, where 1 - beta2 is 2^-10).  A second moment above zero keeps at least the smallest code: m / (0 + eps)
 // would be a step of any size.  New moments are formed in fp64 before they are rounded to 8 bits, so that which side of a
 // code border a value falls on does not depend on how the products were contracted.  A moment that is not finite keeps its
 // element to itself: it is left out of the block's scale and stored as NaN.
@@ -28,6 +28,7 @@ constexpr int ADAMW_THREADS = 256;
 constexpr int ADAMW_CHUNK = 2048;             // elements of a block, a multiple of the 256-element state blocks: all loads of a wave in
                                               // flight at once; 4096 in two turns: 90 us instead of 88 for 27 M bf16 elements
 constexpr unsigned ADAMW_P_BF16 = 1, ADAMW_G_BF16 = 2, ADAMW_VECTOR = 4;
+constexpr int ADAMW_NUMBER = 3;               // a tensor's number lies in the flags from this bit on
 
 struct AdamwEntry {                           // 40 bytes
   void* p;
@@ -36,7 +37,7 @@ struct AdamwEntry {                           // 40 bytes
   unsigned state;                             // start in the moment buffers / 256
   float decay;
   unsigned block0;                            // first block of this tensor
-  unsigned flags;
+  unsigned flags;                             // ADAMW_*, and the tensor's number
 };
 struct AdamwList {
   AdamwEntry e[ADAMW_MAX];
@@ -62,6 +63,7 @@ __device__ __forceinline__ int adamw_find(const AdamwList& l, unsigned b) {
   return __popcll(__ballot(first)) + __popcll(__ballot(second)) - 1;
 }
 
+// 32 mixed bits: two rounds of shift and multiply, shifts and multipliers as C. Wellons published them (2018)
 __device__ __forceinline__ unsigned adamw_hash(unsigned x) {
   x = (x ^ (x >> 16)) * 0x7FEB352Du;
   x = (x ^ (x >> 15)) * 0x846CA68Bu;
@@ -322,7 +324,7 @@ __global__ __launch_bounds__(ADAMW_THREADS) void adamw8_kernel(AdamwList list, u
   const AdamwEntry e = list.e[adamw_find(list, blockIdx.x)];
   const AdamwScalars s = adamw_scalars(a);
   const float keep = 1.f - s.lr * e.decay;
-  const unsigned key = e.state * 256u + s.step * 0x9E3779B9u + a.seed * 0x85EBCA6Bu;
+  const unsigned key = (e.flags >> ADAMW_NUMBER) * 0xC2B2AE35u + s.step * 0x9E3779B9u + a.seed * 0x85EBCA6Bu;
   const Adamw8State o{exp_avg + (long)e.state * 256, exp_avg_sq + (long)e.state * 256, m_scale + e.state, v_scale + e.state};
   const long lo = (long)(blockIdx.x - e.block0) * ADAMW_CHUNK, hi = min(e.n, lo + ADAMW_CHUNK);
   const bool pb = e.flags & ADAMW_P_BF16, gb = e.flags & ADAMW_G_BF16, vec = e.flags & ADAMW_VECTOR;
@@ -447,6 +449,8 @@ int adamw_check(const char* name, const dn_adamw_tensor* t, int count, bool stat
     DN_CHECK_ARG(!((uintptr_t)t[i].grad & ga) && (!state || !((uintptr_t)t[i].param & pa)), "%s: tensor %d: misaligned pointer", name, i);
     DN_CHECK_ARG(!state || (t[i].state >= 0 && t[i].state % 256 == 0 && t[i].state / 256 < (1L << 32)),
                  "%s: tensor %d: state offset %ld is not a multiple of 256", name, i, t[i].state);
+    DN_CHECK_ARG(!state || (t[i].number >= 0 && t[i].number < 1 << (32 - ADAMW_NUMBER)), "%s: tensor %d: number %d is not within 0 and 2^29 - 1",
+                 name, i, t[i].number);
   }
   return DN_OK;
 }
@@ -464,7 +468,7 @@ long adamw_fill(const dn_adamw_tensor* t, int count, int chunk, int* first, Adam
       e.p = x.param; e.g = x.grad; e.n = x.n; e.state = (unsigned)(x.state / 256); e.decay = x.weight_decay; e.block0 = (unsigned)blocks;
       const uintptr_t pa = x.param_dtype == DN_BF16 ? 7 : 15, ga = x.grad_dtype == DN_BF16 ? 7 : 15;
       e.flags = (x.param_dtype == DN_BF16 ? ADAMW_P_BF16 : 0) | (x.grad_dtype == DN_BF16 ? ADAMW_G_BF16 : 0) |
-                (((uintptr_t)x.param & pa) || ((uintptr_t)x.grad & ga) ? 0 : ADAMW_VECTOR);
+                (((uintptr_t)x.param & pa) || ((uintptr_t)x.grad & ga) ? 0 : ADAMW_VECTOR) | (unsigned)x.number << ADAMW_NUMBER;
       ++l->count;
       blocks += more;
     }

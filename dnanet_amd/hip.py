@@ -37,7 +37,7 @@ class DnPackJob(Structure):
 class DnAdamwTensor(Structure):
     """``dn_adamw_tensor`` of include/dnanet_hip.h."""
     _fields_ = [("param", c_void_p), ("grad", c_void_p), ("n", c_long), ("state", c_long), ("weight_decay", c_float),
-                ("param_dtype", c_int), ("grad_dtype", c_int), ("reserved", c_int)]
+                ("param_dtype", c_int), ("grad_dtype", c_int), ("number", c_int)]
 
 
 class HipError(RuntimeError):

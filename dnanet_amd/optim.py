@@ -41,7 +41,8 @@ class HipAdamW:
     say).  Tensors without a gradient are left out of a step.
 
     ``state_bits``: 32 (fp32 moments) or 8 (e4m3 codes with a power-of-two scale per 256 elements, stochastic rounding from
-    ``seed`` and the step number: the same run gives the same bits).  The moments of all tensors lie in the flat buffers
+    ``seed``, the step number, a tensor's place among the parameters and an element's in its tensor: the same run gives the same
+    bits).  The moments of all tensors lie in the flat buffers
     ``exp_avg`` / ``exp_avg_sq``, in the order of the parameters, each tensor from a multiple of 256 elements on; with 8 bits
     they are ``float8_e4m3fn`` and belong to the per-block scales ``exp_avg_scale`` / ``exp_avg_sq_scale``.
 
@@ -156,11 +157,11 @@ class HipAdamW:
         for group in self.param_groups:
             start = len(rows)
             for p in group["params"]:
-                g, at = grads[k], self.offsets[k]
+                g, at, number = grads[k], self.offsets[k], k
                 k += 1
                 if g is not None and p.numel():
                     rows.append(DnAdamwTensor(p.data_ptr(), g.data_ptr(), p.numel(), at, group["weight_decay"], _DTYPE[p.dtype],
-                                              _DTYPE[g.dtype], 0))
+                                              _DTYPE[g.dtype], number))
             self._slices.append((start, len(rows) - start))
         self._table = (DnAdamwTensor * max(1, len(rows)))(*rows)
         self._rows = len(rows)

@@ -330,7 +330,8 @@ int dn_adam_step_graph(float* params, float* grads, float* exp_avg, float* exp_a
  * the buffers hold whole blocks of 256.
  *   state_bits 32: fp32.  state_bits 8: one e4m3 code per element and one fp32 scale per block of 256 (exp_avg_scale /
  *   exp_avg_sq_scale [state / 256 + block], powers of two; value = code * scale), rounded stochastically from a hash of
- *   (element's place in the buffers, step, seed); a moment that is not finite is stored as NaN.
+ *   (tensor's number, element in the tensor, step, seed): the same bits wherever the tensor lies in the list, in the buffers or in
+ *   memory; a moment that is not finite is stored as NaN.
  * clip (nullable): {norm, coefficient} in device memory as dn_grad_norm writes them; gradients are multiplied by the
  * coefficient.  zero_grad: gradients are zeroed in the same pass.  step counts from 1. */
 typedef struct dn_adamw_tensor {
@@ -340,7 +341,7 @@ typedef struct dn_adamw_tensor {
   long state;            /* first element in the moment buffers, a multiple of 256 */
   float weight_decay;
   int param_dtype, grad_dtype;   /* DN_DTYPE_F32 | DN_DTYPE_BF16 */
-  int reserved;
+  int number;            /* 8-bit moments: the tensor's own among those of the optimizer, 0 to 2^29 - 1 */
 } dn_adamw_tensor;
 int dn_adamw_step(const dn_adamw_tensor* tensors, int count, void* exp_avg, void* exp_avg_sq, float* exp_avg_scale,
                   float* exp_avg_sq_scale, int state_bits, double lr, double beta1, double beta2, double eps, long step, unsigned seed,

@@ -39,3 +39,9 @@ def gpu_device():
     if not torch.cuda.is_available():
         pytest.skip("no GPU")
     return torch.device("cuda:0")
+
+
+def pytest_collection_modifyitems(items):
+    """One test holds other rounding bits than the definition has (by place in the moment buffers, not by tensor number and
+    element: see test_adamw_rounding_gpu.py).  It runs, unchanged, behind all others: with ``-x`` its failure hides none of them."""
+    items.sort(key=lambda item: item.nodeid.split("[")[0].endswith("test_adamw_gpu.py::test_8_bit_states"))
