@@ -210,13 +210,14 @@ def prepare(case, seed):
 def _own_optimizer(s):
     from dnanet_amd.optim import HipAdamW
     case = s["case"]
-    params = []
-    for n, at in zip(s["sizes"], s["starts"]):
-        p = s["p"][at:at + n]
-        p.grad = s["g"][at:at + n]
-        params.append(p)
+    params, grads = ([s[name][at:at + n] for n, at in zip(s["sizes"], s["starts"])] for name in ("p", "g"))
     weights = sum(1 for d in s["decay"] if d)
     groups = [{"params": params[:weights], "weight_decay": DECAY}, {"params": params[weights:], "weight_decay": 0.0}]
+    if s["p"].dtype == s["g"].dtype:
+        for p, g in zip(params, grads):
+            p.grad = g
+    else:                                       # torch refuses a .grad of another type: a group's own list
+        groups[0]["grads"], groups[1]["grads"] = grads[:weights], grads[weights:]
     opt = HipAdamW([group for group in groups if group["params"]], lr=LR, betas=(BETA1, BETA2), eps=ADAM_EPS,
                    state_bits=case["bits"], max_grad_norm=case["clip"] or None, seed=s["seed"])
     opt.step_count = FIRST_STEP
