@@ -1,0 +1,11 @@
+// Epochs of a workspace's launches and the tags of the words that they publish there (plain C++: the host can run it).
+//
+// A launch finds the epoch of its workspace (0 at first: the workspace is zero-filled) and publishes its words with the tag
+// epoch + 1, so that no word of an earlier launch, and no word that was never written, has its tag.  The launch's last block
+// leaves the next epoch.  After the last tag, 2^32 - 1, it first zeroes every word and starts again from epoch 0: no tag comes a
+// second time while a word of its first time is there.
+#pragma once
+
+constexpr unsigned gn_epoch_tag(unsigned epoch) { return epoch + 1; }
+constexpr bool gn_last_tag(unsigned tag) { return tag == 0xFFFFFFFFu; }
+constexpr unsigned gn_epoch_after(unsigned tag) { return gn_last_tag(tag) ? 0u : tag; }

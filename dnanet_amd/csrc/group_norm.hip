@@ -16,6 +16,7 @@
 #include <algorithm>
 #include "common.h"
 #include "dnanet_hip.h"
+#include "gn_epoch.h"
 
 namespace {
 
@@ -397,7 +398,8 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const unsigned
 // of 1.4 to 2.1 ms a round, blocks of one launch holding the slots that another's needed.  Clusters kept within an XCD: 216 us.)
 //
 // A published word carries the launch's epoch beside its 32-bit value, so no fence and no clearing is needed: words of earlier
-// launches have other epochs.  The launch's last block counts the epoch up; counters return to zero.
+// launches have other epochs (gn_epoch.h).  The launch's last block counts the epoch up and, when it starts again from 0, zeroes
+// all words; counters return to zero.
 constexpr int GNF_THREADS = 512;
 constexpr int GNF_WAVES = GNF_THREADS / 64;
 // Blocks of a cluster: 64 KB each, so groups (or sets of planes) up to 12 MB of bf16 or fp32.  bf16, one pass against three launches: 64 x 128
@@ -496,7 +498,7 @@ __device__ __forceinline__ bool gnf_place(const GnFused& f, unsigned* missing, G
   u.alone = f.d_most.d == 1;                           // every cluster of the launch is one block: nothing is exchanged
   if (threadIdx.x == 0) *missing = 0;
   const unsigned epoch = u.alone ? 0 : __hip_atomic_load(f.ctrl, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  u.tag = epoch % 0xFFFFFFFFu + 1;                     // never 0, what the workspace is filled with at first
+  u.tag = gn_epoch_tag(epoch);
   return gnf_locate(f, u, blockIdx.x);
 }
 
@@ -595,7 +597,15 @@ __device__ __forceinline__ void gnf_last(const GnFused& f, const GnPlace& u, uns
   gnf_reset(f.ctrl + GNF_LINE);                                                                // the launch's last
   *last = 1;
 }
-// The launch's last block: the next listed place into `u`; false: none is left, the epoch is counted up.  (One barrier.)
+// The launch's last block, done with everything: the next launch's epoch.  All others have read their words by now.
+__device__ __forceinline__ void gnf_next_epoch(const GnFused& f, unsigned tag) {
+  static_assert(GNF_LIST0 + GNF_MAX_BLOCKS * 8L == GNF_SLOT0, "the list and the slots lie together");
+  if (gn_last_tag(tag))                                // once in 2^32 - 1 launches
+    for (long i = threadIdx.x; i < (GNF_END - GNF_LIST0) / 8; i += GNF_THREADS)
+      __hip_atomic_store(f.list + i, 0ULL, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (threadIdx.x == 0) __hip_atomic_store(f.ctrl, gn_epoch_after(tag), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// The launch's last block: the next listed place into `u`; false: none is left.  (One barrier.)
 __device__ __forceinline__ bool gnf_next_listed(const GnFused& f, GnPlace& u, unsigned* at, unsigned* next) {
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -609,7 +619,6 @@ __device__ __forceinline__ bool gnf_next_listed(const GnFused& f, GnPlace& u, un
       *next = (unsigned)v;
     } else {
       gnf_reset(f.ctrl + 2 * GNF_LINE);
-      gnf_count(f.ctrl);
     }
   }
   __syncthreads();
@@ -832,6 +841,7 @@ __global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_kernel(GnFused f, GnF
       gnf_apply<T, ACT, 1, PARTIAL>(o, f.s, u, one, i, sh);
     }
   }
+  gnf_next_epoch(f, u.tag);
 }
 
 // backward: part[block][channel] = (sum dz, sum dz * xhat) for the parameter gradients, group sums as above
@@ -1057,6 +1067,7 @@ __global__ __launch_bounds__(GNF_THREADS, R <= 4 ? 6 : 4) void gn_fused_bwd_kern
       gnf_apply_bwd<T, ACT, 1, false, PARTIAL>(o, s, u, one_g, one_x, i, sh);
     }
   }
+  gnf_next_epoch(f, u.tag);
 }
 
 int gn_shape(const char* name, dn_tensor x, int N, int H, int W, int groups, int dtype, GnShape* out) {
