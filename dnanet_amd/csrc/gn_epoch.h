@@ -9,3 +9,13 @@
 constexpr unsigned gn_epoch_tag(unsigned epoch) { return epoch + 1; }
 constexpr bool gn_last_tag(unsigned tag) { return tag == 0xFFFFFFFFu; }
 constexpr unsigned gn_epoch_after(unsigned tag) { return gn_last_tag(tag) ? 0u : tag; }
+
+// The 32-bit value of a published word {tag, value}: looks at it until its tag is `tag`, `looks` times at most; false: it is not there.
+template <typename Load> constexpr bool gn_take(unsigned tag, int looks, Load load, unsigned* value) {
+  for (; looks > 0; --looks) {
+    const unsigned long long word = load();
+    *value = (unsigned)word;
+    if ((unsigned)(word >> 32) == tag) return true;
+  }
+  return false;
+}

@@ -409,6 +409,7 @@ constexpr int GNF_MAX_K = 192;
 constexpr int GNF_MAX_CELLS = 1024;              // published cells of a cluster
 constexpr int GNF_MAX_BLOCKS = 16384;            // blocks of a launch: more images take more launches
 constexpr int GNF_POLLS = 4096;                  // looks at a word before a block gives up: about 0.6 ms
+constexpr int GNF_SURE = 1 << 16;                // looks at a word that has been stored: about 10 ms
 constexpr int GNF_SHARDS = 16;                   // counters of finished clusters
 constexpr int GNF_LINE = 32;                     // counters 128 bytes apart: epoch, finished shards, listed, then the shards'
 constexpr long GNF_CTRL_BYTES = (3 + GNF_SHARDS) * GNF_LINE * 4L, GNF_DEPART_BYTES = GNF_MAX_BLOCKS * 4L;
@@ -576,11 +577,15 @@ __device__ __forceinline__ bool gnf_collect(const GnFused& f, const GnPlace& u, 
   }
   return !given_up;
 }
-// The launch's last block to wait: everything is there, with or without patience.
+// The launch's last block to wait: all blocks have stored their words, but a word may still be on its way (a block's count of
+// departure is not ordered behind the words that another of its waves stored).  One that never comes makes the result NaN.
 __device__ __forceinline__ void gnf_collect_again(const GnFused& f, const GnPlace& u, float* cells) {
   const unsigned long long* p = f.slot + u.cluster0 * f.ncell * 2;
-  for (int w = threadIdx.x; w < u.k * f.ncell * 2; w += GNF_THREADS)
-    cells[w] = __uint_as_float((unsigned)__hip_atomic_load(p + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  for (int w = threadIdx.x; w < u.k * f.ncell * 2; w += GNF_THREADS) {
+    unsigned value = 0;
+    const bool there = gn_take(u.tag, GNF_SURE, [&] { return __hip_atomic_load(p + w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }, &value);
+    cells[w] = there ? __uint_as_float(value) : __builtin_nanf("");
+  }
   __syncthreads();
 }
 // Whether this block is the launch's last to wait (thread GNF_COUNTER; the answer is for after the next barrier).

@@ -1,4 +1,5 @@
-"""The tags of a group-norm workspace's launches, from the header that the kernels use, compiled for the host."""
+"""The tags of a group-norm workspace's launches, and how its words are read, from the header that the kernels use,
+compiled for the host."""
 import os
 import subprocess
 
@@ -42,3 +43,29 @@ def test_no_tag_comes_twice_while_its_words_are_there(tmp_path):
     assert not mistaken(rows), "words of the first launches are still there when the last tag has come"
     assert mistaken([(e % ((1 << 32) - 1) + 1, False) for e in ((1 << 32) - 2, (1 << 32) - 1, 0, 1)]) == [2], \
         "a tag that epochs 2^32 - 1 and 0 share is found"
+
+
+WORDS = r"""
+#include <cstdio>
+#include "gn_epoch.h"
+using word = unsigned long long;
+int main() {
+  // a word that arrives after `late` looks; before that the word of an earlier launch is there
+  const int late[] = {0, 1, 7, 8, 1000};
+  for (int n : late) {
+    int looks = 0;
+    unsigned value = 0;
+    const bool there = gn_take(5, 8, [&] { return looks++ < n ? (word)4 << 32 | 111 : (word)5 << 32 | 222; }, &value);
+    std::printf("%d %u %d\n", there, value, looks);
+  }
+}
+"""
+
+
+def test_words_of_other_launches_are_not_taken(tmp_path):
+    src, exe = tmp_path / "words.cpp", tmp_path / "words"
+    src.write_text(WORDS)
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(ROOT, "dnanet_amd", "csrc"), str(src), "-o", str(exe)], check=True, timeout=120)
+    got = [tuple(map(int, line.split())) for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=60).stdout.splitlines()]
+    assert got[:3] == [(1, 222, 1), (1, 222, 2), (1, 222, 8)]
+    assert [(there, looks) for there, _, looks in got[3:5]] == [(0, 8), (0, 8)], "bounded, and told apart"
