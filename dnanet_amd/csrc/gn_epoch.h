@@ -19,3 +19,14 @@ template <typename Load> constexpr bool gn_take(unsigned tag, int looks, Load lo
   }
   return false;
 }
+// The next of the listed places from *at on that a block of this launch has put there; `none` if there is none.  Words without the
+// launch's tag, and places that valid(place) refuses, come from a workspace that was not zeroed: they are passed over.
+template <typename Load, typename Valid>
+constexpr unsigned gn_take_listed(unsigned tag, int looks, unsigned listed, unsigned* at, unsigned none, Load load, Valid valid) {
+  while (*at < listed) {
+    const unsigned i = (*at)++;
+    unsigned place = 0;
+    if (gn_take(tag, looks, [&] { return load(i); }, &place) && valid(place)) return place;
+  }
+  return none;
+}

@@ -614,23 +614,16 @@ __device__ __forceinline__ void gnf_next_epoch(const GnFused& f, unsigned tag) {
 __device__ __forceinline__ bool gnf_next_listed(const GnFused& f, GnPlace& u, unsigned* at, unsigned* next) {
   __syncthreads();
   if (threadIdx.x == 0) {
-    *next = 0xFFFFFFFFu;
     if (*at == 0) __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    const unsigned listed = __hip_atomic_load(f.ctrl + 2 * GNF_LINE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (*at < listed && *at < GNF_MAX_BLOCKS) {
-      unsigned long long v = 0;
-      for (int tries = 0; (unsigned)(v >> 32) != u.tag && tries < 1 << 22; ++tries)
-        v = __hip_atomic_load(f.list + *at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      *next = (unsigned)v;
-    } else {
-      gnf_reset(f.ctrl + 2 * GNF_LINE);
-    }
+    const unsigned listed = min((unsigned)GNF_MAX_BLOCKS, __hip_atomic_load(f.ctrl + 2 * GNF_LINE, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    *next = gn_take_listed(
+        u.tag, GNF_SURE, listed, at, gridDim.x, [&](unsigned i) { return __hip_atomic_load(f.list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); },
+        [&](unsigned place) { GnPlace probe; return place < gridDim.x && gnf_locate(f, probe, place); });
+    if (*next == gridDim.x) gnf_reset(f.ctrl + 2 * GNF_LINE);
   }
   __syncthreads();
-  const unsigned v = __builtin_amdgcn_readfirstlane(*next);
-  if (v >= gridDim.x) return false;                    // none (or a workspace that was not zeroed)
-  ++*at;
-  return gnf_locate(f, u, v);
+  const unsigned place = __builtin_amdgcn_readfirstlane(*next);
+  return place < gridDim.x && gnf_locate(f, u, place);
 }
 
 __device__ __forceinline__ void gnf_wave_sum64(double& a, double& b) {

@@ -1,4 +1,4 @@
-"""The tags of a group-norm workspace's launches, and how its words are read, from the header that the kernels use,
+"""The tags of a group-norm workspace's launches, and how its words and its list are read, from the header that the kernels use,
 compiled for the host."""
 import os
 import subprocess
@@ -58,6 +58,12 @@ int main() {
     const bool there = gn_take(5, 8, [&] { return looks++ < n ? (word)4 << 32 | 111 : (word)5 << 32 | 222; }, &value);
     std::printf("%d %u %d\n", there, value, looks);
   }
+  // places 3, (another launch's) 9, (outside the grid) 70, 6; then nothing
+  const word list[] = {(word)5 << 32 | 3, (word)4 << 32 | 9, (word)5 << 32 | 70, (word)5 << 32 | 6};
+  unsigned at = 0;
+  for (int i = 0; i < 3; ++i)
+    std::printf("%u\n", gn_take_listed(5, 8, 4, &at, 64, [&](unsigned k) { return list[k]; }, [](unsigned place) { return place < 64; }));
+  std::printf("%u\n", at);
 }
 """
 
@@ -69,3 +75,4 @@ def test_words_of_other_launches_are_not_taken(tmp_path):
     got = [tuple(map(int, line.split())) for line in subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=60).stdout.splitlines()]
     assert got[:3] == [(1, 222, 1), (1, 222, 2), (1, 222, 8)]
     assert [(there, looks) for there, _, looks in got[3:5]] == [(0, 8), (0, 8)], "bounded, and told apart"
+    assert got[5:] == [(3,), (6,), (64,), (4,)]

@@ -61,3 +61,26 @@ def test_words_of_the_turn_before(gpu_device, dtype):
         got, want = passes(WIDE, dtype, ws, seed), passes(WIDE, dtype, None, seed)
         assert all(torch.equal(x, y) for x, y in zip(got, want)), seed
     assert epoch(ws) == 4
+
+
+# byte offsets in a workspace: the count of listed places, the list
+LISTED, LIST = 2 * 32 * 4, (3 + 16) * 32 * 4 + 16384 * 4 + 4096 * 4
+
+
+@pytest.mark.parametrize("place,tag", [(0xFFFFFFF0, 0), (1 << 20, 0), (0, 0), (0, 1)])
+def test_list_that_no_block_wrote(gpu_device, place, tag):
+    """A list with a place outside the grid, with one that is done already, with one of another launch: all segments are right, the list
+    is empty afterwards and the epoch is the next."""
+    from dnanet_amd.group_norm import group_norm_act
+    ws = workspace(WIDE, "bf16")
+    for launch in range(3):
+        buf, _, gamma, beta = make(WIDE, "bf16", seed=launch, offset=3.0)
+        args = gamma.cuda(), beta.cuda(), WIDE[2], EPS, "relu"
+        want, _ = group_norm_act(buf.ref(WIDE[1]), *args)
+        if launch == 1:
+            ws[LISTED:LISTED + 4].view(torch.int32).fill_(2)
+            words = ws[LIST:LIST + 16].view(torch.int32)
+            words.copy_(torch.tensor([place - (1 << 32) if place >> 31 else place, epoch(ws) + 1 + tag, 1, epoch(ws) + 1], dtype=torch.int32))
+        got, _ = group_norm_act(buf.ref(WIDE[1]), *args, workspace=ws)
+        assert torch.equal(got.data, want.data), launch
+        assert epoch(ws) == launch + 1 and not ws[LISTED:LISTED + 4].any()
