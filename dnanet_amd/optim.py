@@ -7,9 +7,8 @@ tensors with gradients, and optionally clips the gradients to a global norm, whi
 from __future__ import annotations
 
 import ctypes
-import weakref
 from contextlib import nullcontext
-from operator import is_
+from operator import attrgetter
 from typing import Iterable, List, Optional, Sequence, Union
 
 import torch
@@ -22,10 +21,18 @@ _DTYPE = {torch.float32: F32, torch.bfloat16: BF16}
 _BLOCK = 256                     # elements of an 8-bit state block; a tensor's moments start at a multiple of it
 
 
-_data_ptr = torch.Tensor.data_ptr
+_data_ptr, _numel, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+_dtype, _grad = attrgetter("dtype"), attrgetter("grad")
 # torch.cuda.is_current_stream_capturing / current_device without their checks for a driver: 0.6 us of a call of 14
 _capturing, _current_device = torch._C._cuda_isCurrentStreamCapturing, torch._C._cuda_getDevice
 _HERE = nullcontext()
+
+
+def _layout(tensors: List[torch.Tensor]) -> tuple:
+    """Where tensors lie and what their memory holds: a tensor that keeps its address can still become a shorter one, one of
+    another type or a strided one (``p.data = p.data[:k]``, ``resize_``, ``set_``), and a kernel that takes it for what it was writes past
+    its end.  (With addresses alone a step on 44 tensors takes the host 18 us, so 26: torch tells these things one at a time.)"""
+    return list(map(_data_ptr, tensors)), list(map(_numel, tensors)), list(map(_dtype, tensors)), all(map(_is_contiguous, tensors))
 
 
 def _blocks(n: int) -> int:
@@ -85,7 +92,7 @@ class HipAdamW:
                 raise ValueError(f"{len(given)} gradients for {len(group['params'])} parameters")
             self._given += given
             self.param_groups.append(group)
-        self._all_given = all(g is not None for g in self._given)
+        self._all_given, self._none_given = all(g is not None for g in self._given), all(g is None for g in self._given)
         self._params: List[torch.Tensor] = [p for g in self.param_groups for p in g["params"]]
         if not self._params:
             raise ValueError("no parameters")
@@ -116,8 +123,7 @@ class HipAdamW:
             if nbytes < 0:
                 hip.check(1)
             self._partial = torch.empty(nbytes // 8, dtype=torch.float64, device=self.device)
-        self._grads: Sequence = ()               # weak references to the gradients the table below was made for
-        self._pointers: List[int] = []
+        self._made_for: tuple = ()               # layouts and decays that the table below was made for
         self._decays: List[float] = []
         self._table, self._slices = None, []
 
@@ -133,16 +139,24 @@ class HipAdamW:
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("parameters overlap in memory (a tensor listed twice?)")
 
-    # ---- the tensor table: rebuilt when a parameter, a gradient or a decay is another one than last time -----------------
+    # ---- the tensor table: rebuilt when a parameter or a gradient lies elsewhere or is of another kind, or a decay is another one
+    # than last time ---------------------------------------------------------------------------------------------------------
     def _refresh(self):
         decays = [g["weight_decay"] for g in self.param_groups]
         if self._table is not None and self.model is not None and decays == self._decays:
             return                               # a model's arenas stay where they are
-        grads = self._given if self._all_given else [p.grad if g is None else g for p, g in zip(self._params, self._given)]
-        pointers = list(map(_data_ptr, self._params))
-        pointers += map(_data_ptr, grads if self._all_given else [g for g in grads if g is not None])
-        if self._table is not None and pointers == self._pointers and decays == self._decays and \
-                (self._all_given or all(map(is_, grads, [r and r() for r in self._grads]))):
+        if self._all_given:
+            grads = self._given
+        elif self._none_given:
+            grads = list(map(_grad, self._params))
+        else:
+            grads = [p.grad if g is None else g for p, g in zip(self._params, self._given)]
+        try:
+            made_for = _layout(self._params + grads), None, decays
+        except TypeError:                        # tensors without a gradient
+            missing = [g is None for g in grads]
+            made_for = _layout(self._params + [g for g in grads if g is not None]), missing, decays
+        if made_for == self._made_for:
             return
         self._check_params()
         for p, g, n in zip(self._params, grads, self._sizes):
@@ -165,8 +179,7 @@ class HipAdamW:
             self._slices.append((start, len(rows) - start))
         self._table = (DnAdamwTensor * max(1, len(rows)))(*rows)
         self._rows = len(rows)
-        self._grads = [g if g is None else weakref.ref(g) for g in grads]
-        self._pointers, self._decays = pointers, decays
+        self._made_for, self._decays = made_for, decays
 
     def _part(self, start: int):
         return ctypes.cast(ctypes.byref(self._table, start * ctypes.sizeof(DnAdamwTensor)), ctypes.POINTER(DnAdamwTensor))
