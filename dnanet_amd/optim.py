@@ -54,14 +54,13 @@ class HipAdamW:
     they are ``float8_e4m3fn`` and belong to the per-block scales ``exp_avg_scale`` / ``exp_avg_sq_scale``.
 
     ``max_grad_norm``: scale the gradients by ``min(1, max_grad_norm / (norm + 1e-6))`` of their common 2-norm, which is
-    left in ``grad_norm`` (a device scalar); the gradients themselves are not rewritten."""
+    left in ``grad_norm`` (a device scalar); the gradients themselves are not rewritten.  It may be set, changed and taken back (None)
+    between steps."""
 
     def __init__(self, params: Union[ParameterTree, Iterable], lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, state_bits: int = 32, max_grad_norm: Optional[float] = None, seed: int = 0):
         if state_bits not in (32, 8):
             raise ValueError(f"state_bits must be 32 or 8, got {state_bits!r}")
-        if max_grad_norm is not None and not max_grad_norm > 0:
-            raise ValueError(f"max_grad_norm must be above zero, got {max_grad_norm!r}")
         if not 0 <= int(seed) < 1 << 32:
             raise ValueError(f"seed must fit 32 bits, got {seed!r}")
         self.model = params if isinstance(params, ParameterTree) else None
@@ -98,7 +97,7 @@ class HipAdamW:
             raise ValueError("no parameters")
         self.device = getattr(self._params[0], "device", None)
         self._check_params()
-        self.state_bits, self.max_grad_norm, self.seed = state_bits, max_grad_norm, int(seed)
+        self.state_bits, self.seed = state_bits, int(seed)
         self.step_count = 0
         self._zeroed = False
         self._sizes = [p.numel() for p in self._params]
@@ -113,19 +112,30 @@ class HipAdamW:
         self.exp_avg_scale = self.exp_avg_sq_scale = None
         if state_bits == 8:
             self.exp_avg_scale, self.exp_avg_sq_scale = (torch.zeros(at // _BLOCK, dtype=torch.float32, device=self.device) for _ in range(2))
-        self._clip = self._partial = self.grad_norm = None
-        if max_grad_norm is not None:
-            self._clip = torch.zeros(2, dtype=torch.float32, device=self.device)
-            self.grad_norm = self._clip[0]
+        self._clip = self._partial = None
+        self.max_grad_norm = max_grad_norm
+        self._made_for: tuple = ()               # layouts and decays that the table below was made for
+        self._decays: List[float] = []
+        self._table, self._slices = None, []
+
+    @property
+    def max_grad_norm(self) -> Optional[float]:
+        return self._max_grad_norm
+
+    @max_grad_norm.setter
+    def max_grad_norm(self, value: Optional[float]):
+        if value is not None and not value > 0:
+            raise ValueError(f"max_grad_norm must be above zero, got {value!r}")
+        if value is not None and self._clip is None:         # kept from then on: a captured step may hold them
             # sizes count here, pointers only have to be some
             whole = (DnAdamwTensor * len(self._params))(*[DnAdamwTensor(4096, 4096, n, 0, 0.0, F32, F32, 0) for n in self._sizes])
             nbytes = hip.lib.dn_grad_norm_workspace_bytes(whole, len(self._params))
             if nbytes < 0:
                 hip.check(1)
             self._partial = torch.empty(nbytes // 8, dtype=torch.float64, device=self.device)
-        self._made_for: tuple = ()               # layouts and decays that the table below was made for
-        self._decays: List[float] = []
-        self._table, self._slices = None, []
+            self._clip = torch.zeros(2, dtype=torch.float32, device=self.device)
+        self._max_grad_norm = value
+        self.grad_norm = None if value is None else self._clip[0]
 
     def _check_params(self):
         spans = []
@@ -211,9 +221,9 @@ class HipAdamW:
         with guard:
             stream = hip.raw_stream(self.device)
             clip = None
-            if self._clip is not None:
+            if self._max_grad_norm is not None:
                 clip = self._clip.data_ptr()
-                hip.check(lib.dn_grad_norm(self._table, self._rows, self.max_grad_norm, clip, self._partial.data_ptr(),
+                hip.check(lib.dn_grad_norm(self._table, self._rows, self._max_grad_norm, clip, self._partial.data_ptr(),
                                            self._partial.numel() * 8, stream))
             if device_state is not None:
                 hyper, step = device_state
