@@ -189,6 +189,7 @@ class HipAdamW:
             self._slices.append((start, len(rows) - start))
         self._table = (DnAdamwTensor * max(1, len(rows)))(*rows)
         self._rows = len(rows)
+        self._written = [p for p, g in zip(self._params, grads) if g is not None]
         self._made_for, self._decays = made_for, decays
 
     def _part(self, start: int):
@@ -238,7 +239,7 @@ class HipAdamW:
             self.model._param_epoch += 1
             self._zeroed = True
         elif not capturing:
-            torch.autograd.graph.increment_version(self._params)     # the kernel's writes are in-place updates to autograd
+            torch.autograd.graph.increment_version(self._written)    # the kernel's writes are in-place updates to autograd
 
     def zero_grad(self, set_to_none: bool = True):
         """A model's gradient arena was zeroed by ``step`` itself; ``.grad`` tensors are dropped (or zeroed), a group's own
