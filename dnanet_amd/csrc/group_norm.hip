@@ -602,15 +602,13 @@ __device__ __forceinline__ void gnf_last(const GnFused& f, const GnPlace& u, uns
   gnf_reset(f.ctrl + GNF_LINE);                                                                // the launch's last
   *last = 1;
 }
-// The launch's last block, done with everything: the next launch's epoch.  All others have read their words by now.
-__device__ __forceinline__ void gnf_next_epoch(const GnFused& f, unsigned tag) {
+// The launch's last block, done with everything, after the last tag: all words are zeroed.  All others have read theirs by now.
+__device__ __noinline__ void gnf_clear_words(unsigned long long* words) {
   static_assert(GNF_LIST0 + GNF_MAX_BLOCKS * 8L == GNF_SLOT0, "the list and the slots lie together");
-  if (gn_last_tag(tag))                                // once in 2^32 - 1 launches
-    for (long i = threadIdx.x; i < (GNF_END - GNF_LIST0) / 8; i += GNF_THREADS)
-      __hip_atomic_store(f.list + i, 0ULL, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  if (threadIdx.x == 0) __hip_atomic_store(f.ctrl, gn_epoch_after(tag), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (long i = threadIdx.x; i < (GNF_END - GNF_LIST0) / 8; i += GNF_THREADS)
+    __hip_atomic_store(words + i, 0ULL, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-// The launch's last block: the next listed place into `u`; false: none is left.  (One barrier.)
+// The launch's last block: the next listed place into `u`; false: none is left, and the next launch's epoch is there.
 __device__ __forceinline__ bool gnf_next_listed(const GnFused& f, GnPlace& u, unsigned* at, unsigned* next) {
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -619,7 +617,10 @@ __device__ __forceinline__ bool gnf_next_listed(const GnFused& f, GnPlace& u, un
     *next = gn_take_listed(
         u.tag, GNF_SURE, listed, at, gridDim.x, [&](unsigned i) { return __hip_atomic_load(f.list + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); },
         [&](unsigned place) { GnPlace probe; return place < gridDim.x && gnf_locate(f, probe, place); });
-    if (*next == gridDim.x) gnf_reset(f.ctrl + 2 * GNF_LINE);
+    if (*next == gridDim.x) {
+      gnf_reset(f.ctrl + 2 * GNF_LINE);
+      __hip_atomic_store(f.ctrl, gn_epoch_after(u.tag), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
   }
   __syncthreads();
   const unsigned place = __builtin_amdgcn_readfirstlane(*next);
@@ -839,7 +840,7 @@ __global__ __launch_bounds__(GNF_THREADS, 6) void gn_fused_kernel(GnFused f, GnF
       gnf_apply<T, ACT, 1, PARTIAL>(o, f.s, u, one, i, sh);
     }
   }
-  gnf_next_epoch(f, u.tag);
+  if (gn_last_tag(u.tag)) gnf_clear_words(f.list);
 }
 
 // backward: part[block][channel] = (sum dz, sum dz * xhat) for the parameter gradients, group sums as above
@@ -1065,7 +1066,7 @@ __global__ __launch_bounds__(GNF_THREADS, R <= 4 ? 6 : 4) void gn_fused_bwd_kern
       gnf_apply_bwd<T, ACT, 1, false, PARTIAL>(o, s, u, one_g, one_x, i, sh);
     }
   }
-  gnf_next_epoch(f, u.tag);
+  if (gn_last_tag(u.tag)) gnf_clear_words(f.list);
 }
 
 int gn_shape(const char* name, dn_tensor x, int N, int H, int W, int groups, int dtype, GnShape* out) {
