@@ -49,7 +49,7 @@ CONV35_FLOP_H5 = 57_271_910_400       # the eighteen 3x5 convolutions of the for
 FIRST_FLOP_H5 = 19_660_800            # encoders.0 conv1 (1 -> 32): taps are the K dimension, nothing is skipped
 BF16_PEAK_TFLOPS = 2500.0             # dense bf16 MFMA peak, MI355X_MICROARCH.md
 F32_PEAK_TFLOPS = 157.3
-TRAFFIC_PROFILE = os.path.join(ROOT, "profiles", "r03_traffic.json")
+TRAFFIC_PROFILE = os.path.join(ROOT, "profiles", "current_traffic.json")
 
 
 def parse_args(argv=None):
@@ -165,7 +165,7 @@ def cpu_baseline(rows: int, seconds_budget: float = 24.0):
 # ---------------------------------------------------------------------------------------------------------------------
 # GPU legs
 # ---------------------------------------------------------------------------------------------------------------------
-# what the kernels behind a bench tag are compiled from (profiles/r03_traffic.json records the hash of these files)
+# what the kernels behind a bench tag are compiled from (profiles/current_traffic.json records the hash of these files)
 TRAFFIC_SOURCES = {
     "conv_igemm": ["conv_igemm.h", "common.h", "api.hip", "conv_inst_bf16_k35.hip", "conv_inst_f32_k35.hip"],
     "conv_igemm8": ["conv_igemm8.h", "conv_igemm.h", "common.h", "api.hip", "conv8_inst_bf16.hip", "conv8_inst_f32.hip"],

@@ -1,6 +1,6 @@
-"""Turn the rocprofv3 output of scratch/profile_bench.sh (gpurun_out/r03_<dtype>/) into the committed files of profiles/.
+"""Turn the rocprofv3 output of scratch/profile_bench.sh (gpurun_out/<tag>_<dtype>/) into the committed files of profiles/.
 
-    python scratch/make_profiles.py [round tag, default r03]
+    python scratch/make_profiles.py [tag, default current]
 
 Per precision (fp32 = the headline, bf16): kernel statistics of the inference-only run, of the run with the training leg
 (two streams, and one stream: the time base for per-kernel figures of the training step), the JSON lines those runs
@@ -12,7 +12,7 @@ from collections import defaultdict
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 G, P = os.path.join(ROOT, "gpurun_out"), os.path.join(ROOT, "profiles")
-tag = sys.argv[1] if len(sys.argv) > 1 else "r03"
+tag = sys.argv[1] if len(sys.argv) > 1 else "current"
 sys.path.insert(0, ROOT)
 from bench import kernel_source_digest, TRAFFIC_SOURCES  # noqa: E402
 

@@ -1,15 +1,16 @@
 #!/bin/bash
-# rocprofv3 passes over bench.py (round 3): for the headline precision (fp32) and for bf16 --
+# rocprofv3 passes over bench.py: for the headline precision (fp32) and for bf16 --
 #   kernel stats of the inference leg alone and with the training leg, HBM fetch / write counters and matrix-core counters in
 #   runs of their own (with the training leg, so the training kernels have figures too), and a single-stream kernel trace
 #   (DN_TUNE_NO_WGRAD_STREAM=1: with the weight gradients on a second stream, overlapping kernels stretch each other).
-# Results under gpurun_out/; scratch/make_profiles.py turns them into profiles/.   usage: profile_bench.sh [fp32|bf16]
+# Results under gpurun_out/; scratch/make_profiles.py turns them into profiles/.   usage: profile_bench.sh [fp32|bf16] [tag, default current]
 set -e
 R=$GRAFT_REPO_ROOT
 DT=${1:-fp32}
+TAG=${2:-current}
 cd /tmp && export TMPDIR=/tmp
 B="--dtype $DT --no-cpu-baseline --no-legs"
-O=$R/gpurun_out/r03_$DT
+O=$R/gpurun_out/${TAG}_$DT
 mkdir -p $O
 timeout -k 10 300 rocprofv3 --kernel-trace --stats -d $O/prof_infer -o p --output-format csv -- python3 $R/bench.py --steps 10 $B --no-train > $O/prof_infer_bench.log 2>&1
 timeout -k 10 400 rocprofv3 --kernel-trace --stats -d $O/prof_full -o p --output-format csv -- python3 $R/bench.py --steps 10 $B > $O/prof_full_bench.log 2>&1
