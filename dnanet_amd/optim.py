@@ -14,6 +14,7 @@ from typing import Iterable, List, Optional, Sequence, Union
 import torch
 
 from . import hip
+from ._layout import layout as _layout      # built from csrc/tensor_layout.cpp
 from .hip import BF16, F32, DnAdamwTensor
 from .params import ParameterTree
 
@@ -21,18 +22,10 @@ _DTYPE = {torch.float32: F32, torch.bfloat16: BF16}
 _BLOCK = 256                     # elements of an 8-bit state block; a tensor's moments start at a multiple of it
 
 
-_data_ptr, _numel, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
-_dtype, _grad = attrgetter("dtype"), attrgetter("grad")
+_grad = attrgetter("grad")
 # torch.cuda.is_current_stream_capturing / current_device without their checks for a driver: 0.6 us of a call of 14
 _capturing, _current_device = torch._C._cuda_isCurrentStreamCapturing, torch._C._cuda_getDevice
 _HERE = nullcontext()
-
-
-def _layout(tensors: List[torch.Tensor]) -> tuple:
-    """Where tensors lie and what their memory holds: a tensor that keeps its address can still become a shorter one, one of
-    another type or a strided one (``p.data = p.data[:k]``, ``resize_``, ``set_``), and a kernel that takes it for what it was writes past
-    its end.  (With addresses alone a step on 44 tensors takes the host 18 us, so 26: torch tells these things one at a time.)"""
-    return list(map(_data_ptr, tensors)), list(map(_numel, tensors)), list(map(_dtype, tensors)), all(map(_is_contiguous, tensors))
 
 
 def _blocks(n: int) -> int:
@@ -161,11 +154,9 @@ class HipAdamW:
             grads = list(map(_grad, self._params))
         else:
             grads = [p.grad if g is None else g for p, g in zip(self._params, self._given)]
-        try:
-            made_for = _layout(self._params + grads), None, decays
-        except TypeError:                        # tensors without a gradient
-            missing = [g is None for g in grads]
-            made_for = _layout(self._params + [g for g in grads if g is not None]), missing, decays
+        # not the addresses alone: a tensor that keeps its own can become shorter, strided or one of another type (``p.data = p.data[:k]``,
+        # ``resize_``, ``set_``), and a kernel that takes it for what it was writes past its end
+        made_for = _layout(self._params + grads), decays
         if made_for == self._made_for:
             return
         self._check_params()

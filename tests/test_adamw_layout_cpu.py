@@ -36,3 +36,11 @@ def test_layout_tells_tensors_at_one_address_apart(change, which):
     assert _layout(tensors) == before
     change(tensors[which])
     assert tensors[which].data_ptr() == address and _layout(tensors) != before
+
+
+def test_layout_of_missing_and_foreign_entries():
+    from dnanet_amd.optim import _layout
+    a, b = torch.zeros(4), torch.zeros(4)
+    assert len({_layout(x) for x in ([a, None], [None, a], [a], [a, b], [b, a], [None, None], [])}) == 7
+    with pytest.raises(TypeError, match="tensor or None"):
+        _layout([a, 3])
