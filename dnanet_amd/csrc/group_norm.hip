@@ -382,8 +382,8 @@ __global__ __launch_bounds__(GN_THREADS) void gn_bwd_apply_kernel(const unsigned
 // ---- one pass: the blocks of a group hold its values in registers and exchange their sums --------------------------------
 // The smallest traffic a group norm can have is one read and one write (backward: two reads and one write); statistics in a launch
 // of their own cost a second read of all of it: 234 us forward and 382 us backward for the sizes below.  This form is bound by
-// HBM: 256 x 32 x 6 x 4096 bf16 forward 177 us for 0.81 GB (4.5 TB/s, a copy of as many bytes takes 152), 256 x 512 x 6 x 256 backward
-// 275 us for 1.21 GB (4.4 TB/s; 228); the vector units are busy for half of that time, and the waits for other blocks are hidden
+// HBM: 256 x 32 x 6 x 4096 bf16 forward 176 us for 0.81 GB (4.6 TB/s, a copy of as many bytes takes 152), 256 x 512 x 6 x 256 backward
+// 271 us for 1.21 GB (4.5 TB/s; 228); the vector units are busy for half of that time, and the waits for other blocks are hidden
 // behind the other one or two blocks of the CU.  Small calls are bound by the exchange: 2 x 128 x 5 x 64 fp32 8 us on the device.
 // Here a block keeps its segment in registers, publishes the segment's sums, waits for those of the other blocks of its
 // cluster -- the segments of the planes whose channels form whole groups -- and finishes from registers.
@@ -404,7 +404,8 @@ constexpr int GNF_THREADS = 512;
 constexpr int GNF_WAVES = GNF_THREADS / 64;
 // Blocks of a cluster: 64 KB each, so groups (or sets of planes) up to 12 MB of bf16 or fp32.  bf16, one pass against three launches: 64 x 128
 // channels of one group x 6 x 4096 (96 blocks) forward 217 / 240 us, backward 320 / 370; 32 x 256 channels (192 blocks) 226 / 251 and 365 / 376; 32 x 512
-// channels (384 blocks) 488 / 488 and 884 / 720: there a CU's two blocks wait for a whole chip of others.
+// channels (384 blocks) 488 / 488 and 884 / 720: there a CU's two blocks wait for a whole chip of others.  A cluster's cells have to fit
+// the LDS as well: at most 1024 / (cells of a plane) blocks, 64 for bf16 groups of an odd number of channels.
 constexpr int GNF_MAX_K = 192;
 constexpr int GNF_MAX_CELLS = 1024;              // published cells of a cluster
 constexpr int GNF_MAX_BLOCKS = 16384;            // blocks of a launch: more images take more launches
@@ -712,7 +713,7 @@ __device__ __forceinline__ void gnf_scales(const GnFused& f, const GnForward& o,
     const float mean32 = (float)(pivot + shift);
     const float var = (float)((s2 - s1 * shift) * f.inv_total + (double)o.eps);
     float rstd = __builtin_amdgcn_rsqf(var);
-    rstd = fmaf(rstd * 0.5f, fmaf(-var * rstd, rstd, 1.f), rstd);                // one Newton step
+    rstd = fmaf(rstd * 0.5f, fmaf(-var * rstd, rstd, 1.f), rstd);                // one Newton step (three launches: a fp64 root)
     if (lane == 0) {
       sh.gstat[g - g_lo][0] = mean32;
       sh.gstat[g - g_lo][1] = rstd;

@@ -21,9 +21,8 @@ from .params import ParameterTree
 _DTYPE = {torch.float32: F32, torch.bfloat16: BF16}
 _BLOCK = 256                     # elements of an 8-bit state block; a tensor's moments start at a multiple of it
 
-
 _grad = attrgetter("grad")
-# torch.cuda.is_current_stream_capturing / current_device without their checks for a driver: 0.6 us of a call of 14
+# torch.cuda.is_current_stream_capturing / current_device without their checks for a driver: 0.6 us of a call of 13
 _capturing, _current_device = torch._C._cuda_isCurrentStreamCapturing, torch._C._cuda_getDevice
 _HERE = nullcontext()
 
